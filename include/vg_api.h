@@ -23,7 +23,7 @@ extern "C" {
 
 enum { VG_F32 = 0, VG_BF16 = 1 };
 enum { VG_OK = 0, VG_ERR_BAD_ARG = -1, VG_ERR_HIP = -2, VG_ERR_UNSUPPORTED = -3 };
-enum { VG_ACT_NONE = 0, VG_ACT_LRELU = 1, VG_ACT_SIGMOID = 2 };
+enum { VG_ACT_NONE = 0, VG_ACT_LRELU = 1, VG_ACT_SIGMOID = 2, VG_ACT_GELU = 3 /* z Phi(z) */, VG_ACT_SILU = 4 }; /* 3, 4: vg_linear_act_* only */
 
 #define VG_STATS_REPLICAS 32 /* per-channel f64 accumulators are spread over this many copies */
 
@@ -383,6 +383,55 @@ int vg_augment_batch(const vg_aug_item* items, int n, int out_h, int out_w, void
  * descriptor) stays for every other shape. */
 int vg_linear_wgrad(const float* x, const float* gy, float* dw, int b, int fin, int fout, int accumulate, void* stream);
 int vg_linear_dgrad(const float* gy, const float* w, float* dx, int b, int fin, int fout, void* stream);
+
+/* ---- token-wise operators of a model of the code indices (no counterpart in the reference, which stops at the index map) ----
+ * Layer norm over the first c of cs columns; rows have a stride of ldx / ldy elements; columns c..cs-1 of y and dx are
+ * written as zeros.  y = (x - mean) * rstd * w + b.  stats: [rows][2] f32 out (mean, 1/sqrt(var + eps)), NULL without a
+ * backward pass.  w, b, dw, db f32; x, y, dy, dx in `dtype`.  rows < 2^31. */
+int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, int64_t ldy, float* stats, int64_t rows, int c,
+                      int cs, float eps, int dtype, void* stream);
+/* dx, and dw / db (either may be NULL) through per-block partial sums in ws (vg_layer_norm_bwd_ws_bytes), added in a fixed
+ * order: the same bits on every run. */
+size_t vg_layer_norm_bwd_ws_bytes(int64_t rows, int c);
+int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* w, const float* stats, void* dx, int64_t lddx,
+                      float* dw, float* db, void* ws, int64_t rows, int c, int cs, int dtype, void* stream);
+
+/* y = act(x W^T + bias) + res: x [m][k] (row stride ldx), w [n][k], y [m][n]; bias [n] in bias_dtype (`dtype` or VG_F32) or
+ * NULL; res [m][n] (row stride ldres) or NULL; z: NULL, or [m][n] for x W^T + bias, which the backward pass of an activation
+ * needs.  f32 accumulation. */
+int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, const void* bias, int bias_dtype, const void* res, int64_t ldres, void* y,
+                      void* z, int64_t m, int64_t n, int64_t k, int act, int dtype, void* stream);
+/* dz = dy * act'(z) (not written for VG_ACT_NONE: dz is dy) and db = its column sums, taken before dz is rounded (NULL: not wanted;
+ * otherwise ws of vg_linear_act_dz_ws_bytes). */
+size_t vg_linear_act_dz_ws_bytes(int64_t m, int64_t n);
+int vg_linear_act_dz(const void* dy, const void* z, void* dz, void* db, int bias_dtype, void* ws, int64_t m, int64_t n, int act, int dtype,
+                     void* stream);
+/* dx [m][k] = dz w;  dw [n][k] = dz^T x, in dw_dtype (`dtype` or VG_F32). */
+int vg_linear_act_dgrad(const void* dz, const void* w, void* dx, int64_t m, int64_t n, int64_t k, int dtype, void* stream);
+int vg_linear_act_wgrad(const void* dz, const void* x, int64_t ldx, void* dw, int dw_dtype, int64_t m, int64_t n, int64_t k, int dtype,
+                        void* stream);
+
+/* Log probability of tokens[r] under row r of logits [rows][vocab] (row stride ldx), the row's entropy (nats) and its `top` best
+ * alternatives (0..32; by value, then by lower place).  lse: [rows][2] f32 out for the backward pass, or NULL.  -inf logits are
+ * masked; a row of only -inf gives logp -inf, entropy 0, gradient 0; NaN or +inf in a row gives NaN (a NaN ranks as -inf among the
+ * alternatives).  tokens[r] == ignore: logp 0 and no gradient through it; another token outside [0, vocab): logp NaN, no gradient
+ * through it.  ws: vg_token_logprobs_ws_bytes (0: none needed). */
+size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top);
+int vg_token_logprobs_fwd(const void* logits, int64_t ldx, const int64_t* tokens, int64_t ignore, int64_t rows, int vocab, int top,
+                          float* logp, float* entropy, float* lse, float* top_logp, int64_t* top_at, void* ws, int dtype, void* stream);
+/* d logits of sum_r dlogp[r] logp[r] + dent[r] entropy[r] (either gradient may be NULL). */
+int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* tokens, int64_t ignore, const float* lse, const float* entropy,
+                          const float* dlogp, const float* dent, void* dx, int64_t lddx, int64_t rows, int vocab, int dtype, void* stream);
+
+/* AdamW (decoupled weight decay) over a flat buffer of n elements, n a multiple of 256, every tensor begun at a multiple of 256:
+ *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  p = p (1 - lr wd) - lr / (1-b1^step) * m / (sqrt(v / (1-b2^step)) + eps)
+ * g is multiplied by grad_scale first.  decay: [n / 256] bytes, 0 = the block's tensor is not decayed; NULL: all are.
+ * The 8-bit form keeps m and sqrt(v) as e4m3 codes with one f32 scale per 256 elements (largest magnitude / 448). */
+int vg_adamw_step(float* p, const float* g, float* m, float* v, const unsigned char* decay, int64_t n, double lr, double beta1, double beta2,
+                  double eps, double weight_decay, int step, float grad_scale, void* stream);
+int vg_adamw8_step(float* p, const float* g, void* m_codes, float* m_scale, void* r_codes, float* r_scale, const unsigned char* decay,
+                   int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay, int step, float grad_scale,
+                   void* stream);
 
 #ifdef __cplusplus
 }

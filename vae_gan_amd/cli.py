@@ -10,6 +10,8 @@ Every reference flag keeps its name, type, default and meaning: ``--output_dir -
   --bn_sync {local,global}           data parallel only: BatchNorm / VQ-EMA statistics per rank, or of the global batch
   --recon_target_policy {error,area} 'error' raises like beta_vae_gans/model.py:255; 'area' is shim D1
   --hier_decoder_policy {error,nearest}  'error' raises like hierarchical_vae_gan/model.py:261; 'nearest' is shim D2
+  --optimizer {adam,adamw,adamw8bit} 'adam' is the reference's; 'adamw' decays weights by --weight_decay (default 0.01),
+                                     'adamw8bit' also keeps its moments in 8 bits
   --image_size N                     Config.image_size (the reference has no flag for it)
   --num_workers N                    Config.num_workers (PNG-decoding loader processes; the reference has no flag)
   --max_iters N                      stop every epoch after N iterations (smoke runs)
@@ -61,6 +63,9 @@ def build_parser(arch: str) -> argparse.ArgumentParser:
     if arch == "hier":
         p.add_argument('--hier_decoder_policy', choices=('error', 'nearest'), default='error',
                        help="'error' raises like the reference's decoder, 'nearest' chains the sub-blocks with nearest x2")
+    p.add_argument('--optimizer', choices=('adam', 'adamw', 'adamw8bit'), default='adam',
+                   help='adam: the reference; adamw: decoupled weight decay; adamw8bit: the same with 8-bit states')
+    p.add_argument('--weight_decay', type=float, default=0.01, help='weight decay of adamw / adamw8bit (weights only)')
     p.add_argument('--image_size', type=int, default=None, help='Config.image_size (default: the config value, 256)')
     p.add_argument('--num_workers', type=int, default=None, help='Config.num_workers (default: the config value, 4)')
     p.add_argument('--max_iters', type=int, default=None, help='stop each epoch after this many iterations')
@@ -81,6 +86,7 @@ def config_from_args(arch: str, args):
     for n in ("output_dir", "data_dir", "batch_size", "epochs", "lambda_adv") + names:
         setattr(config, n, getattr(args, n))
     config.recon_target_policy = args.recon_target_policy
+    config.optimizer, config.weight_decay = args.optimizer, args.weight_decay
     if arch == "hier":
         config.hier_decoder_policy = args.hier_decoder_policy
     if args.image_size is not None:

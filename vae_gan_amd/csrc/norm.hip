@@ -1,0 +1,393 @@
+// Layer norm over the last dimension, forward and backward, and the column reduction that its parameter gradients (and the
+// bias gradient of vg_linear_act_dz) end in.
+//   mu = sum x / c, var = sum (x - mu)^2 / c, r = (var + eps)^-1/2, xh = (x - mu) r, y = xh w + b
+//   g = dy w:  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+// Rows are [c valid + padding] elements with a row stride; padding columns of y / dx are written as zeros (the NHWC
+// convention).  Bound by memory: x is read and y written once; backward reads x and dy and writes dx once.  A row is held
+// in the registers of GL lanes (a part of a wave, a wave, or the block's four waves) as NV accesses of VEC elements, so the
+// variance is that of the centred values (no cancellation of sum(x^2) - mu^2) at no second read.  All sums are f32.
+#include "common.h"
+#include "rows.h"
+
+
+template <typename T, int VEC> __device__ __forceinline__ void ld_vec(const T* p, float* o) {
+  typedef T vt __attribute__((ext_vector_type(VEC)));
+  if constexpr (VEC == 1) o[0] = (float)*p;
+  else {
+    const vt v = *(const vt*)p;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = (float)v[e];
+  }
+}
+template <typename T, int VEC> __device__ __forceinline__ void st_vec(T* p, const float* o) {
+  typedef T vt __attribute__((ext_vector_type(VEC)));
+  if constexpr (VEC == 1) *p = (T)o[0];
+  else {
+    vt v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (T)o[e];
+    *(vt*)p = v;
+  }
+}
+
+// sum over the GL lanes that share a row; every lane gets it.  GL == 256: through LDS (red: one slot per wave and value)
+template <int GL> __device__ __forceinline__ float row_sum(float v, float* red, int slot) {
+#pragma unroll
+  for (int o = (GL < 64 ? GL : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (GL > 64) {
+    if ((threadIdx.x & 63) == 0) red[slot * 4 + (threadIdx.x >> 6)] = v;
+    __syncthreads();
+    v = (red[slot * 4] + red[slot * 4 + 1]) + (red[slot * 4 + 2] + red[slot * 4 + 3]);
+  }
+  return v;
+}
+
+template <typename T, int VEC, int GL, int NV>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
+                                                     const float* __restrict__ b, T* __restrict__ y, int64_t ldy,
+                                                     float* __restrict__ stats, int64_t rows, int c, int cs, float eps) {
+  __shared__ float red[8];
+  constexpr int RPB = 256 / GL;
+  const int gl = threadIdx.x % GL;
+  const int64_t row = blockIdx.x * (int64_t)RPB + threadIdx.x / GL;
+  const bool live = row < rows;                       // dead groups still take part in the shuffles and barriers
+  float v[NV][VEC];
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * GL + gl) * VEC;
+    if (live && col < cs) ld_vec<T, VEC>(x + row * ldx + col, v[i]);
+    else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s += col + e < c ? v[i][e] : 0.f;
+  }
+  const float inv = 1.f / (float)c;
+  const float mu = row_sum<GL>(s, red, 0) * inv;
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * GL + gl) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = v[i][e] - mu;
+      q += col + e < c ? d * d : 0.f;
+    }
+  }
+  const float var = row_sum<GL>(q, red, 1) * inv;
+  const float r = 1.f / sqrtf(var + eps);
+  if (!live) return;
+  if (stats && gl == 0) { stats[2 * row] = mu; stats[2 * row + 1] = r; }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * GL + gl) * VEC;
+    if (col >= cs) break;
+    float o[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const bool in = col + e < c;
+      o[e] = in ? (v[i][e] - mu) * r * w[in ? col + e : 0] + b[in ? col + e : 0] : 0.f;
+    }
+    st_vec<T, VEC>(y + row * ldy + col, o);
+  }
+}
+
+// rows too long for the registers of a block: three passes over the row (the second and third come from the caches)
+template <typename T>
+__global__ __launch_bounds__(256) void ln_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
+                                                          const float* __restrict__ b, T* __restrict__ y, int64_t ldy,
+                                                          float* __restrict__ stats, int c, int cs, float eps) {
+  __shared__ float red[8];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < c; i += 256) s += (float)xr[i];
+  const float mu = row_sum<256>(s, red, 0) / (float)c;
+  float q = 0.f;
+  for (int i = threadIdx.x; i < c; i += 256) { const float d = (float)xr[i] - mu; q += d * d; }
+  const float r = 1.f / sqrtf(row_sum<256>(q, red, 1) / (float)c + eps);
+  if (stats && threadIdx.x == 0) { stats[2 * row] = mu; stats[2 * row + 1] = r; }
+  for (int i = threadIdx.x; i < cs; i += 256) y[row * ldy + i] = (T)(i < c ? ((float)xr[i] - mu) * r * w[i] + b[i] : 0.f);
+}
+
+// dx of the rows of this block (block-strided), and the block's partial sums of dw and db: part[block][2][c]
+template <typename T, int VEC, int GL, int NV>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
+                                                     const float* __restrict__ w, const float* __restrict__ stats,
+                                                     T* __restrict__ dx, int64_t lddx, float* __restrict__ part, int64_t rows,
+                                                     int c, int cs) {
+  __shared__ float red[16];
+  extern __shared__ float fold[];                    // [waves][GL x VEC] for the last fold (GL <= 64)
+  constexpr int RPB = 256 / GL;
+  const int gl = threadIdx.x % GL;
+  const float inv = 1.f / (float)c;
+  float aw[NV][VEC], ab[NV][VEC], wv[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int col = (i * GL + gl) * VEC + e;
+      aw[i][e] = ab[i][e] = 0.f;
+      wv[i][e] = col < c ? w[col] : 0.f;
+    }
+  int turn = 0;
+  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 2) {
+    const int64_t row = r0 + threadIdx.x / GL;
+    const bool live = row < rows;
+    float xh[NV][VEC], g[NV][VEC];
+    const float mu = live ? stats[2 * row] : 0.f, r = live ? stats[2 * row + 1] : 0.f;
+    float sg = 0.f, sgx = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * GL + gl) * VEC;
+      if (live && col < cs) {
+        ld_vec<T, VEC>(x + row * ldx + col, xh[i]);
+        ld_vec<T, VEC>(dy + row * lddy + col, g[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) xh[i][e] = g[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * GL + gl) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const bool in = live && col + e < c;
+        xh[i][e] = in ? (xh[i][e] - mu) * r : 0.f;
+        g[i][e] = in ? g[i][e] : 0.f;
+        aw[i][e] += g[i][e] * xh[i][e];
+        ab[i][e] += g[i][e];
+        g[i][e] *= wv[i][e];
+        sg += g[i][e];
+        sgx += g[i][e] * xh[i][e];
+      }
+    }
+    // two LDS slots in turn: a wave can be one row ahead of the readers of the other pair
+    const float mg = row_sum<GL>(sg, red, turn) * inv, mgx = row_sum<GL>(sgx, red, turn + 1) * inv;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * GL + gl) * VEC;
+        if (col >= cs) break;
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = col + e < c ? r * (g[i][e] - mg - xh[i][e] * mgx) : 0.f;
+        st_vec<T, VEC>(dx + row * lddx + col, o);
+      }
+    }
+  }
+  if (!part) return;
+  float* pw = part + (size_t)blockIdx.x * 2 * c;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int col = (i * GL + gl) * VEC + e;
+      float a = aw[i][e], d = ab[i][e];
+      if constexpr (GL < 64) {
+#pragma unroll
+        for (int o = GL; o < 64; o <<= 1) { a += __shfl_xor(a, o, 64); d += __shfl_xor(d, o, 64); }
+      }
+      if constexpr (GL <= 64) {                      // fold the block's four waves in a fixed order
+        __syncthreads();
+        if ((threadIdx.x & 63) < GL) { fold[(threadIdx.x >> 6) * GL + gl] = a; fold[(4 + (threadIdx.x >> 6)) * GL + gl] = d; }
+        __syncthreads();
+        if (threadIdx.x < GL && col < c) {
+          pw[col] = (fold[gl] + fold[GL + gl]) + (fold[2 * GL + gl] + fold[3 * GL + gl]);
+          pw[c + col] = (fold[4 * GL + gl] + fold[5 * GL + gl]) + (fold[6 * GL + gl] + fold[7 * GL + gl]);
+        }
+      } else if (col < c) { pw[col] = a; pw[c + col] = d; }
+    }
+}
+
+// long rows: dx row by row; the parameter gradients by columns in a kernel of their own
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
+                                                          const float* __restrict__ w, const float* __restrict__ stats,
+                                                          T* __restrict__ dx, int64_t lddx, int c, int cs) {
+  __shared__ float red[8];
+  const int64_t row = blockIdx.x;
+  const T *xr = x + row * ldx, *dr = dy + row * lddy;
+  const float mu = stats[2 * row], r = stats[2 * row + 1];
+  float sg = 0.f, sgx = 0.f;
+  for (int i = threadIdx.x; i < c; i += 256) {
+    const float g = (float)dr[i] * w[i];
+    sg += g;
+    sgx += g * (((float)xr[i] - mu) * r);
+  }
+  const float mg = row_sum<256>(sg, red, 0) / (float)c, mgx = row_sum<256>(sgx, red, 1) / (float)c;
+  for (int i = threadIdx.x; i < cs; i += 256)
+    dx[row * lddx + i] = (T)(i < c ? r * ((float)dr[i] * w[i] - mg - ((float)xr[i] - mu) * r * mgx) : 0.f);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_long_params_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
+                                                                 int64_t lddy, const float* __restrict__ stats,
+                                                                 float* __restrict__ part, int64_t rows, int c, int64_t rows_per) {
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col >= c) return;
+  const int64_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < rows ? r0 + rows_per : rows;
+  float a = 0.f, d = 0.f;
+  for (int64_t r = r0; r < r1; ++r) {
+    const float g = (float)dy[r * lddy + col];
+    a += g * (((float)x[r * ldx + col] - stats[2 * r]) * stats[2 * r + 1]);
+    d += g;
+  }
+  part[(size_t)blockIdx.y * 2 * c + col] = a;
+  part[(size_t)blockIdx.y * 2 * c + c + col] = d;
+}
+
+// out[col] = sum over parts of part[p][col], in the order of p within each of 8 interleaved groups, then the groups in order
+template <typename O>
+__global__ __launch_bounds__(256) void fold_cols_kernel(const float* __restrict__ part, int parts, int64_t cols, int64_t stride,
+                                                        O* __restrict__ out0, int64_t split, O* __restrict__ out1) {
+  __shared__ float s[8][32];
+  const int cx = threadIdx.x & 31, py = threadIdx.x >> 5;
+  const int64_t col = blockIdx.x * (int64_t)32 + cx;
+  float a = 0.f;
+  if (col < cols)
+    for (int p = py; p < parts; p += 8) a += part[p * stride + col];
+  s[py][cx] = a;
+  __syncthreads();
+  if (py == 0 && col < cols) {
+    float t = s[0][cx];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += s[i][cx];
+    O* o = col < split ? out0 + col : out1 + (col - split);
+    if (col < split ? out0 != nullptr : out1 != nullptr) *o = (O)t;
+  }
+}
+
+int vg_fold_cols(const float* part, int parts, int64_t cols, void* out0, int64_t split, void* out1, int dtype, hipStream_t st) {
+  const dim3 grid((unsigned)vg_ceil_div(cols, 32));
+  if (dtype == VG_BF16)
+    hipLaunchKernelGGL(fold_cols_kernel<bf16_t>, grid, dim3(256), 0, st, part, parts, cols, cols, (bf16_t*)out0, split, (bf16_t*)out1);
+  else hipLaunchKernelGGL(fold_cols_kernel<float>, grid, dim3(256), 0, st, part, parts, cols, cols, (float*)out0, split, (float*)out1);
+  VG_LAUNCH_CHECK();
+  return VG_OK;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+// blocks of the backward pass: enough to fill the chip, few enough that the partial sums (8 c bytes a block) stay small
+static int64_t ln_bwd_blocks(int64_t rows, int rpb) {
+  const int64_t need = vg_ceil_div(rows, rpb);
+  return need < 1024 ? need : 1024;
+}
+static const int LN_LONG_PARTS = 64;
+
+static bool aligned16(const void* p, int64_t ld, int elt) { return (uintptr_t)p % 16 == 0 && (ld * elt) % 16 == 0; }
+
+struct LnArgs {
+  const void *x, *dy;
+  int64_t ldx, lddy, ldo;
+  const float *w, *b;
+  void* out;
+  float *stats, *part;
+  int64_t rows;
+  int c, cs;
+  float eps;
+};
+
+template <typename T, int VEC, int GL, int NV> static void ln_launch(const LnArgs& a, bool bwd, hipStream_t st) {
+  constexpr int RPB = 256 / GL;
+  if (!bwd)
+    hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, GL, NV>), dim3((unsigned)vg_ceil_div(a.rows, RPB)), dim3(256), 0, st, (const T*)a.x,
+                       a.ldx, a.w, a.b, (T*)a.out, a.ldo, a.stats, a.rows, a.c, a.cs, a.eps);
+  else
+    hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, GL, NV>), dim3((unsigned)ln_bwd_blocks(a.rows, RPB)), dim3(256),
+                       GL <= 64 ? 8 * GL * sizeof(float) : 0, st, (const T*)a.x, a.ldx, (const T*)a.dy, a.lddy, a.w, a.stats,
+                       (T*)a.out, a.ldo, a.part, a.rows, a.c, a.cs);
+}
+
+// The lanes that share a row: the fewest whose VEC-element accesses cover it, so that narrow rows (a 41-channel latent) do
+// not leave most of a wave idle; from one wave up the accesses per lane grow first (no barrier), then the whole block.
+// Returns the number of parts, 0 for rows that do not fit (the long kernels).
+template <typename T, int VEC> static int ln_dispatch(const LnArgs& a, bool bwd, bool go, hipStream_t st) {
+  const int n = (int)vg_ceil_div(a.cs, VEC);          // accesses a row needs
+#define LN_CASE(GL, NV)                                                   \
+  if (n <= GL * NV) {                                                     \
+    if (go) ln_launch<T, VEC, GL, NV>(a, bwd, st);                        \
+    return (int)ln_bwd_blocks(a.rows, 256 / GL);                          \
+  }
+  if constexpr (VEC > 1) {
+    LN_CASE(8, 1) LN_CASE(16, 1) LN_CASE(32, 1) LN_CASE(64, 1) LN_CASE(64, 2) LN_CASE(64, 4)
+    if constexpr (VEC == 4) { LN_CASE(64, 8) LN_CASE(256, 4) LN_CASE(256, 8) }
+    else { LN_CASE(256, 2) LN_CASE(256, 4) }
+  } else {
+    LN_CASE(16, 4) LN_CASE(64, 4) LN_CASE(64, 16) LN_CASE(64, 32) LN_CASE(256, 16) LN_CASE(256, 32)
+  }
+#undef LN_CASE
+  return 0;
+}
+template <typename T> static int ln_dispatch_t(const LnArgs& a, bool bwd, bool go, bool vec, hipStream_t st) {
+  return vec ? ln_dispatch<T, Elt<T>::PIECE>(a, bwd, go, st) : ln_dispatch<T, 1>(a, bwd, go, st);
+}
+static bool ln_vec(const LnArgs& a, int dtype, bool bwd) {
+  const int e = vg_elt_size(dtype);
+  return a.cs % (16 / e) == 0 && aligned16(a.x, a.ldx, e) && aligned16(a.out, a.ldo, e) && (!bwd || aligned16(a.dy, a.lddy, e));
+}
+
+static int ln_check(const char* what, int64_t rows, int c, int cs, int64_t ld0, int64_t ld1, int dtype) {
+  VG_REQUIRE(dtype == VG_F32 || dtype == VG_BF16, "%s: dtype %d", what, dtype);
+  VG_REQUIRE(rows >= 0 && rows < (1LL << 31) && c >= 1 && cs >= c, "%s: %ld rows of %d columns, %d stored", what, (long)rows, c, cs);
+  VG_REQUIRE(ld0 >= cs && ld1 >= cs, "%s: a row stride below the row's %d columns", what, cs);
+  return VG_OK;
+}
+
+extern "C" int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, int64_t ldy, float* stats,
+                                 int64_t rows, int c, int cs, float eps, int dtype, void* stream) {
+  if (int rc = ln_check("layer_norm_fwd", rows, c, cs, ldx, ldy, dtype)) return rc;
+  if (rows == 0) return VG_OK;
+  VG_REQUIRE(x && w && b && y, "layer_norm_fwd: null pointer");
+  VG_REQUIRE(eps >= 0.f, "layer_norm_fwd: eps %g", (double)eps);
+  hipStream_t st = (hipStream_t)stream;
+  LnArgs a = {x, nullptr, ldx, 0, ldy, w, b, y, stats, nullptr, rows, c, cs, eps};
+  const bool vec = ln_vec(a, dtype, false);
+  const int got = dtype == VG_BF16 ? ln_dispatch_t<bf16_t>(a, false, true, vec, st) : ln_dispatch_t<float>(a, false, true, vec, st);
+  if (!got) {
+    if (dtype == VG_BF16)
+      hipLaunchKernelGGL(ln_fwd_long_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, (const bf16_t*)x, ldx, w, b, (bf16_t*)y, ldy, stats, c, cs, eps);
+    else hipLaunchKernelGGL(ln_fwd_long_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, (const float*)x, ldx, w, b, (float*)y, ldy, stats, c, cs, eps);
+  }
+  VG_LAUNCH_CHECK();
+  return VG_OK;
+}
+
+extern "C" size_t vg_layer_norm_bwd_ws_bytes(int64_t rows, int c) {
+  // the most blocks any variant launches; long rows use LN_LONG_PARTS
+  int64_t parts = rows < 1024 ? rows : 1024;
+  if (parts < LN_LONG_PARTS) parts = LN_LONG_PARTS;
+  return (size_t)parts * 2 * (size_t)c * sizeof(float);
+}
+
+extern "C" int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* w, const float* stats,
+                                 void* dx, int64_t lddx, float* dw, float* db, void* ws, int64_t rows, int c, int cs, int dtype,
+                                 void* stream) {
+  if (int rc = ln_check("layer_norm_bwd", rows, c, cs, ldx, lddy, dtype)) return rc;
+  VG_REQUIRE(lddx >= cs, "layer_norm_bwd: a row stride below the row's %d columns", cs);
+  VG_REQUIRE(rows > 0 && x && dy && w && stats && dx, "layer_norm_bwd: null pointer or no rows");
+  VG_REQUIRE((!dw && !db) || ws, "layer_norm_bwd: the parameter gradients need a workspace");
+  hipStream_t st = (hipStream_t)stream;
+  float* part = dw || db ? (float*)ws : nullptr;
+  LnArgs a = {x, dy, ldx, lddy, lddx, w, nullptr, dx, (float*)stats, part, rows, c, cs, 0.f};
+  const bool vec = ln_vec(a, dtype, true);
+  int parts = dtype == VG_BF16 ? ln_dispatch_t<bf16_t>(a, true, true, vec, st) : ln_dispatch_t<float>(a, true, true, vec, st);
+  if (!parts) {
+    parts = rows < LN_LONG_PARTS ? (int)rows : LN_LONG_PARTS;
+    const int64_t per = vg_ceil_div(rows, parts);
+    parts = (int)vg_ceil_div(rows, per);
+    const dim3 grid((unsigned)vg_ceil_div(c, 256), (unsigned)parts);
+    if (dtype == VG_BF16) {
+      hipLaunchKernelGGL(ln_bwd_long_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, (const bf16_t*)x, ldx, (const bf16_t*)dy, lddy, w, stats, (bf16_t*)dx, lddx, c, cs);
+      if (part) hipLaunchKernelGGL(ln_bwd_long_params_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)x, ldx, (const bf16_t*)dy, lddy, stats, part, rows, c, per);
+    } else {
+      hipLaunchKernelGGL(ln_bwd_long_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, (const float*)x, ldx, (const float*)dy, lddy, w, stats, (float*)dx, lddx, c, cs);
+      if (part) hipLaunchKernelGGL(ln_bwd_long_params_kernel<float>, grid, dim3(256), 0, st, (const float*)x, ldx, (const float*)dy, lddy, stats, part, rows, c, per);
+    }
+  }
+  VG_LAUNCH_CHECK();
+  if (part) return vg_fold_cols(part, parts, 2 * (int64_t)c, dw, c, db, VG_F32, st);
+  return VG_OK;
+}

@@ -15,7 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libvg_hip.so")
 
 VG_F32, VG_BF16 = 0, 1
-ACT_NONE, ACT_LRELU, ACT_SIGMOID = 0, 1, 2
+ACT_NONE, ACT_LRELU, ACT_SIGMOID, ACT_GELU, ACT_SILU = 0, 1, 2, 3, 4     # GELU, SILU: linear_act only
 STATS_REPLICAS = 32
 
 
@@ -120,6 +120,19 @@ SIGNATURES = {
     "vg_gamma_residual_bwd": (_I, [_P, _P, _P, _P, _P, _L, _P]),
     "vg_cast": (_I, [_P, _P, _L, _I, _I, _P]),
     "vg_adam_step": (_I, [_P, _P, _P, _P, _L, _F, _F, _F, _F, _I, _F, _P]),
+    "vg_layer_norm_fwd": (_I, [_P, _L, _P, _P, _P, _L, _P, _L, _I, _I, _F, _I, _P]),
+    "vg_layer_norm_bwd_ws_bytes": (C.c_size_t, [_L, _I]),
+    "vg_layer_norm_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _P]),
+    "vg_linear_act_fwd": (_I, [_P, _L, _P, _P, _I, _P, _L, _P, _P, _L, _L, _L, _I, _I, _P]),
+    "vg_linear_act_dz_ws_bytes": (C.c_size_t, [_L, _L]),
+    "vg_linear_act_dz": (_I, [_P, _P, _P, _P, _I, _P, _L, _L, _I, _I, _P]),
+    "vg_linear_act_dgrad": (_I, [_P, _P, _P, _L, _L, _L, _I, _P]),
+    "vg_linear_act_wgrad": (_I, [_P, _P, _L, _P, _I, _L, _L, _L, _I, _P]),
+    "vg_token_logprobs_ws_bytes": (C.c_size_t, [_L, _I, _I]),
+    "vg_token_logprobs_fwd": (_I, [_P, _L, _P, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P]),
+    "vg_token_logprobs_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
+    "vg_adamw_step": (_I, [_P, _P, _P, _P, _P, _L, _D, _D, _D, _D, _D, _I, _F, _P]),
+    "vg_adamw8_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _D, _D, _D, _D, _D, _I, _F, _P]),
     "vg_augment_ws_bytes": (C.c_size_t, [_AP, _I, _I, _I]),
     "vg_augment_batch": (_I, [_AP, _I, _I, _I, _P, C.c_size_t, _P, _P]),
     "vg_codebook_usage": (_I, [_P, _L, _I, _I, _P, _P, _P]),

@@ -97,6 +97,33 @@ class BatchNorm2d(nn.Module):
         return self.run(x, None)
 
 
+class LayerNorm(nn.Module):
+    """Layer norm over the channels of NHWC activations (their padding stays zero) or over the last dimension of token rows."""
+
+    def __init__(self, num_features, eps=1e-5):
+        super().__init__()
+        self.num_features, self.eps = num_features, eps
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features))
+
+    def forward(self, x):
+        return ops.layer_norm(x, self.weight, self.bias, self.eps, self.num_features)
+
+
+class LinearAct(nn.Module):
+    """``act(x W^T + b) + residual`` on token rows of the compute dtype, f32 master weights (ops.linear_act)."""
+
+    def __init__(self, in_features, out_features, bias=True, act=L.ACT_NONE):
+        super().__init__()
+        self.in_features, self.out_features, self.act = in_features, out_features, act
+        bound = 1 / math.sqrt(in_features)
+        self.weight = nn.Parameter(torch.empty(out_features, in_features).uniform_(-bound, bound))
+        self.bias = nn.Parameter(torch.empty(out_features).uniform_(-bound, bound)) if bias else None
+
+    def forward(self, x, residual=None):
+        return ops.linear_act(x, self.weight, self.bias, self.act, residual)
+
+
 class LeakyReLU(nn.Module):
     """Marker for LeakyReLU(0.2): always fused into the preceding conv / BatchNorm kernel."""
 

@@ -6,6 +6,7 @@ that is all-reduced in a few large slices on a side stream while nothing else wa
 from __future__ import annotations
 
 import contextlib
+import functools
 import os
 from typing import Optional
 
@@ -13,14 +14,24 @@ import torch
 import torch.distributed as dist
 
 from . import ops
-from .optim import FlatAdam, StepLR
+from .optim import FlatAdam, FlatAdamW, StepLR
 
 
 def build_optimizers(model, config):
-    """<arch>/main.py:34-48: Adam(encoder+decoder, lr) and Adam(discriminator, lr/2), betas from the config."""
-    opt_g = FlatAdam(list(model.encoder.parameters()) + list(model.decoder.parameters()), lr=config.lr,
-                     betas=(config.beta1, config.beta2))
-    opt_d = FlatAdam(model.discriminator.parameters(), lr=config.lr / 2, betas=(config.beta1, config.beta2))
+    """<arch>/main.py:34-48: Adam(encoder+decoder, lr) and Adam(discriminator, lr/2), betas from the config.
+    ``config.optimizer`` (not the reference's): 'adam' (default), 'adamw' or 'adamw8bit', with ``config.weight_decay`` on
+    every parameter of more than one dimension (not on biases and norm weights)."""
+    kind = getattr(config, "optimizer", "adam")
+    if kind == "adam":
+        make = FlatAdam
+    elif kind in ("adamw", "adamw8bit"):
+        make = functools.partial(FlatAdamW, weight_decay=getattr(config, "weight_decay", 0.01), decay_filter=lambda p: p.dim() > 1,
+                                 state_bits=8 if kind == "adamw8bit" else 32)
+    else:
+        raise ValueError(f"config.optimizer must be 'adam', 'adamw' or 'adamw8bit', got {kind!r}")
+    opt_g = make(list(model.encoder.parameters()) + list(model.decoder.parameters()), lr=config.lr,
+                 betas=(config.beta1, config.beta2))
+    opt_d = make(model.discriminator.parameters(), lr=config.lr / 2, betas=(config.beta1, config.beta2))
     return opt_g, opt_d, StepLR(opt_g, 30, 0.5), StepLR(opt_d, 30, 0.5)
 
 
