@@ -396,20 +396,25 @@ size_t vg_layer_norm_bwd_ws_bytes(int64_t rows, int c);
 int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* w, const float* stats, void* dx, int64_t lddx,
                       float* dw, float* db, void* ws, int64_t rows, int c, int cs, int dtype, void* stream);
 
-/* y = act(x W^T + bias) + res: x [m][k] (row stride ldx), w [n][k], y [m][n]; bias [n] in bias_dtype (`dtype` or VG_F32) or
- * NULL; res [m][n] (row stride ldres) or NULL; z: NULL, or [m][n] for x W^T + bias, which the backward pass of an activation
- * needs.  f32 accumulation. */
-int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, const void* bias, int bias_dtype, const void* res, int64_t ldres, void* y,
-                      void* z, int64_t m, int64_t n, int64_t k, int act, int dtype, void* stream);
-/* dz = dy * act'(z) (not written for VG_ACT_NONE: dz is dy) and db = its column sums, taken before dz is rounded (NULL: not wanted;
+/* y = act(x W^T + bias) + res: x [m][k] (row stride ldx), w [n][k] in w_dtype (`dtype`, or VG_F32: rounded to `dtype` for the
+ * products), y [m][n]; bias [n] in bias_dtype (`dtype` or VG_F32) or NULL; res [m][n] (row stride ldres) or NULL.  slope: NULL, or
+ * [m][n] for act'(x W^T + bias), which the backward pass of an activation needs (2 bytes each (f16) for VG_BF16, f32 for VG_F32).
+ * f32 accumulation.  n, k < 2^20.  ws: the bytes that the _ws_bytes function names for the same operands (NULL for 0), aligned to 256. */
+size_t vg_linear_act_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype);
+int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int w_dtype, const void* bias, int bias_dtype, const void* res,
+                      int64_t ldres, void* y, void* slope, void* ws, int64_t m, int64_t n, int64_t k, int act, int dtype, void* stream);
+/* dz = dy * slope (slope NULL: dz is dy and not written) and db = its column sums, taken before dz is rounded (NULL: not wanted;
  * otherwise ws of vg_linear_act_dz_ws_bytes). */
 size_t vg_linear_act_dz_ws_bytes(int64_t m, int64_t n);
-int vg_linear_act_dz(const void* dy, const void* z, void* dz, void* db, int bias_dtype, void* ws, int64_t m, int64_t n, int act, int dtype,
+int vg_linear_act_dz(const void* dy, const void* slope, void* dz, void* db, int bias_dtype, void* ws, int64_t m, int64_t n, int dtype,
                      void* stream);
 /* dx [m][k] = dz w;  dw [n][k] = dz^T x, in dw_dtype (`dtype` or VG_F32). */
-int vg_linear_act_dgrad(const void* dz, const void* w, void* dx, int64_t m, int64_t n, int64_t k, int dtype, void* stream);
-int vg_linear_act_wgrad(const void* dz, const void* x, int64_t ldx, void* dw, int dw_dtype, int64_t m, int64_t n, int64_t k, int dtype,
+size_t vg_linear_act_dgrad_ws_bytes(const void* dz, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype);
+int vg_linear_act_dgrad(const void* dz, const void* w, int w_dtype, void* dx, void* ws, int64_t m, int64_t n, int64_t k, int dtype,
                         void* stream);
+size_t vg_linear_act_wgrad_ws_bytes(const void* dz, const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k, int dtype);
+int vg_linear_act_wgrad(const void* dz, const void* x, int64_t ldx, void* dw, int dw_dtype, void* ws, int64_t m, int64_t n, int64_t k,
+                        int dtype, void* stream);
 
 /* Log probability of tokens[r] under row r of logits [rows][vocab] (row stride ldx), the row's entropy (nats) and its `top` best
  * alternatives (0..32; by value, then by lower place).  lse: [rows][2] f32 out for the backward pass, or NULL.  -inf logits are

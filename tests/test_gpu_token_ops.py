@@ -194,7 +194,10 @@ def la_oracle(x, w, b, res, dy, act, dt):
     if dy is not None:
         d = dy.double().reshape(m, n)
         (dz,) = torch.autograd.grad(a, zz, d)
-        e_slope = BEND[act] * (half(dt) * z.abs() + ez) + (16 * U * (1 + z.abs()) if act != "none" else 0 * z)
+        (slope,) = torch.autograd.grad(act_oracle(zz, act), zz, torch.ones_like(z))
+        # act' goes through f16 (half a step 2^-11 relative, 2^-25 for its subnormals) beside bf16 tensors, f32 beside f32
+        stored = half(torch.float16) * slope.abs() + 2.0 ** -25 if dt == BF16 else U * slope.abs()
+        e_slope = BEND[act] * ez + (stored + 16 * U * (1 + z.abs()) if act != "none" else 0 * z)
         if act == "lrelu":
             e_slope = e_slope + 0.8 * (z.abs() <= ez)                # the sign may flip
         e_dz = d.abs() * e_slope

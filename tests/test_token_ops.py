@@ -131,10 +131,20 @@ def test_c_entry_points_return_an_error_instead_of_launching(ops):
     refused(ln(rows=1 << 31), "rows")
     assert ln(rows=0, x=None) == 0
     refused(lib.vg_layer_norm_bwd(one, 8, one, 8, one, one, one, 8, one, None, None, 1, 8, 8, 0, None), "workspace")
-    refused(lib.vg_linear_act_fwd(one, 7, one, None, 0, None, 0, one, None, 1, 4, 8, 0, 0, None), "row stride")
-    refused(lib.vg_linear_act_fwd(one, 8, one, None, 0, None, 0, one, None, 0, 4, 8, 0, 0, None), "0 x 4 x 8")
-    refused(lib.vg_linear_act_fwd(one, 8, one, None, 0, None, 0, one, None, 1, 4, 8, 7, 0, None), "activation")
-    refused(lib.vg_linear_act_dz(one, None, one, None, 0, None, 1, 4, 3, 0, None), "null")
+    la = lambda **k: lib.vg_linear_act_fwd(*[{**dict(x=one, ldx=8, w=one, wdt=0, b=None, bdt=0, r=None, ldr=0, y=one, s=None, ws=None, m=1, n=4,   # noqa: E731
+                                                     k=8, act=0, dt=0, st=None), **k}[q] for q in "x ldx w wdt b bdt r ldr y s ws m n k act dt st".split()])
+    refused(la(ldx=7), "row stride")
+    refused(la(m=0), "0 x 4 x 8")
+    refused(la(n=1 << 20), "1048576")
+    refused(la(act=7), "activation")
+    refused(la(wdt=1), "weight dtype")
+    refused(la(r=one, ldr=3), "row stride")
+    refused(la(k=7), "workspace")                      # rows that are not whole 16-byte pieces are copied first
+    refused(la(ws=one, k=7), "256")
+    refused(lib.vg_linear_act_dz(one, None, one, None, 0, None, 1, 4, 0, None), "null")
+    refused(lib.vg_linear_act_dz(one, one, one, one, 0, None, 1, 4, 0, None), "null")
+    refused(lib.vg_linear_act_dgrad(one, None, 0, one, None, 1, 4, 8, 0, None), "null")
+    refused(lib.vg_linear_act_wgrad(one, one, 7, one, 0, None, 1, 4, 8, 0, None), "row stride")
     refused(lib.vg_token_logprobs_fwd(one, 8, one, -100, 1, 8, 9, one, one, None, one, one, None, 0, None), "alternatives")
     refused(lib.vg_token_logprobs_fwd(one, 7, one, -100, 1, 8, 0, one, one, None, None, None, None, 0, None), "stride")
     refused(lib.vg_token_logprobs_fwd(one, 1 << 20, one, -100, 1, 1 << 20, 0, one, one, None, None, None, None, 0, None), "workspace")

@@ -1,43 +1,50 @@
 // y = act(x W^T + b) + res and its gradient, x [M][K] and W [N][K] row-major, bf16 or f32, accumulated in f32 on the matrix
-// cores.  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  dres = dy.  z = x W^T + b is stored beside y when a
-// gradient will be wanted (act' of a stored z: one rounding of z to the storage type).
-// All three products are C[i][j] = sum_k A(i, k) B(j, k) with element strides for i / j and k, so one kernel takes any of
-// them, any alignment and any row stride.
+// cores.  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  dres = dy.
+// The forward stores act'(z) beside y when a gradient will be wanted (in f16 for bf16 tensors: 2^-12 relative, where a z or a
+// slope rounded to bf16 would add an error as large as the gradient's own rounding).
+// All three products are C[i][j] = sum_k A(i, k) B(j, k), each operand either with k contiguous (x, W, dz in the first two)
+// or with i / j contiguous (W in dx = dz W, both in dW): a tile of the first kind is read from LDS with 16-byte reads, one of
+// the second with transposing reads, so nothing is transposed in memory.
 #include "common.h"
 #include "rows.h"
 
-__device__ __forceinline__ float la_act(float z, int act) {
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef _Float16 f16_t;
+
+// act(z) and act'(z), sharing the exponential
+__device__ __forceinline__ float la_act(float z, int act, float* slope) {
+  float y = z, s = 1.f;
   switch (act) {
-    case VG_ACT_LRELU: return z > 0.f ? z : VG_LRELU_SLOPE * z;
-    case VG_ACT_SIGMOID: return 1.f / (1.f + __expf(-z));
-    case VG_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case VG_ACT_SILU: return z / (1.f + __expf(-z));
-    default: return z;
+    case VG_ACT_LRELU: s = z > 0.f ? 1.f : VG_LRELU_SLOPE; y = z * s; break;
+    case VG_ACT_SIGMOID: y = 1.f / (1.f + __expf(-z)); s = y * (1.f - y); break;
+    case VG_ACT_GELU: {
+      const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+      y = z * phi;
+      s = phi + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+      break;
+    }
+    case VG_ACT_SILU: { const float p = 1.f / (1.f + __expf(-z)); y = z * p; s = p * (1.f + z * (1.f - p)); break; }
+    default: break;
   }
-}
-__device__ __forceinline__ float la_slope(float z, int act) {
-  switch (act) {
-    case VG_ACT_LRELU: return z > 0.f ? 1.f : VG_LRELU_SLOPE;
-    case VG_ACT_SIGMOID: { const float p = 1.f / (1.f + __expf(-z)); return p * (1.f - p); }
-    case VG_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
-    case VG_ACT_SILU: { const float p = 1.f / (1.f + __expf(-z)); return p * (1.f + z * (1.f - p)); }
-    default: return 1.f;
-  }
+  *slope = s;
+  return y;
 }
 
 struct GemmParams {
   const void *a, *b;
-  int64_t ai, ak, bj, bk;       // element strides
+  int64_t lda, ldb;             // elements between rows of the stored matrix ([m][k] or, transposed, [k][m])
   int m, n, k;
-  void* c;                      // [m][n] out, row stride ldc
-  int64_t ldc;
+  void* c;                      // [m][n] out, row stride n
   int c_f32;                    // C is f32 although the operands are bf16 (gradient of an f32 master weight)
   const void* bias;             // [n] or null
   int bias_f32;
   const void* res;              // [m][n], row stride ldres, or null
   int64_t ldres;
-  void* z;                      // [m][n] pre-activation out, or null
+  void* slope;                  // [m][n] act'(z) out (f16 for bf16, f32 for f32), or null
   int act;
+  int vec;                      // c, res, slope, bias rows take 16-byte accesses
+  float* part;                  // split k: [splits][m][ldp] f32 partial sums instead of C
+  int splits, ldp, ktiles;      // ktiles: of one split
 };
 
 template <typename T> __device__ __forceinline__ f32x4 la_mma(u32x4 a, u32x4 b, f32x4 c);
@@ -52,65 +59,268 @@ template <> __device__ __forceinline__ f32x4 la_mma<float>(u32x4 a, u32x4 b, f32
   return c;
 }
 
-// one output element through the epilogue
-template <typename T> __device__ __forceinline__ void la_store(const GemmParams& p, int i, int j, float v) {
-  if (p.bias) v += p.bias_f32 ? ((const float*)p.bias)[j] : (float)((const T*)p.bias)[j];
-  if (p.z) ((T*)p.z)[(int64_t)i * p.n + j] = (T)v;
-  v = la_act(v, p.act);
-  if (p.res) v += (float)((const T*)p.res)[(int64_t)i * p.ldres + j];
-  if (p.c_f32) ((float*)p.c)[(int64_t)i * p.ldc + j] = v;
-  else ((T*)p.c)[(int64_t)i * p.ldc + j] = (T)v;
+// ---- epilogue: eight neighbouring sums of row i, columns j.. -----------------------------------------------------------
+template <typename T> struct SlopeT;
+template <> struct SlopeT<bf16_t> { typedef f16_t type; };
+template <> struct SlopeT<float> { typedef float type; };
+template <typename O> __device__ __forceinline__ void put8(O* p, const float* v) {
+  typedef O vt __attribute__((ext_vector_type(8)));
+  vt o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (O)v[e];
+  *(vt*)p = o;
 }
-
-// 64 x 64 tile, 4 waves of 32 x 32, 64 bytes of k a step, element loads with bounds
-template <typename T> __global__ __launch_bounds__(256) void gemm_any_kernel(const GemmParams p) {
-  constexpr int KT = 64 / sizeof(T), LD = KT + 16 / sizeof(T), PER = 64 * KT / 256;
-  __shared__ __attribute__((aligned(16))) T sa[64 * LD], sb[64 * LD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tn = (p.n + 63) / 64;
-  const int i0 = (int)(blockIdx.x / tn) * 64, j0 = (int)(blockIdx.x % tn) * 64;
-  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-  const T *A = (const T*)p.a, *B = (const T*)p.b;
-  f32x4 acc[2][2] = {};
-  for (int k0 = 0; k0 < p.k; k0 += KT) {
+template <typename O> __device__ __forceinline__ void get8(const O* p, float* v) {
+  typedef O vt __attribute__((ext_vector_type(8)));
+  const vt o = *(const vt*)p;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int q = tid + e * 256;
-      // neighbouring threads take neighbouring memory
-      const int ra = p.ak == 1 ? q / KT : q % 64, ka = p.ak == 1 ? q % KT : q / 64;
-      const int rb = p.bk == 1 ? q / KT : q % 64, kb = p.bk == 1 ? q % KT : q / 64;
-      sa[ra * LD + ka] = i0 + ra < p.m && k0 + ka < p.k ? A[(i0 + ra) * p.ai + (k0 + ka) * p.ak] : (T)0.f;
-      sb[rb * LD + kb] = j0 + rb < p.n && k0 + kb < p.k ? B[(j0 + rb) * p.bj + (k0 + kb) * p.bk] : (T)0.f;
+  for (int e = 0; e < 8; ++e) v[e] = (float)o[e];
+}
+template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v) {
+  typedef typename SlopeT<T>::type S;
+  const int64_t o = (int64_t)i * p.n + j;
+  if (p.vec && j + 8 <= p.n) {
+    float t[8], s[8];
+    if (p.bias) {
+      if (p.bias_f32) get8((const float*)p.bias + j, t); else get8((const T*)p.bias + j, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
     }
-    __syncthreads();
-    const int off = (lane & 15) * LD + (lane >> 4) * (16 / (int)sizeof(T));
-    u32x4 fa[2], fb[2];
+    if (p.act != VG_ACT_NONE) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      fa[u] = *(const u32x4*)(sa + (wi + u * 16) * LD + off);
-      fb[u] = *(const u32x4*)(sb + (wj + u * 16) * LD + off);
+      for (int e = 0; e < 8; ++e) v[e] = la_act(v[e], p.act, &s[e]);
+      if (p.slope) put8((S*)p.slope + o, s);
     }
+    if (p.res) {
+      get8((const T*)p.res + (int64_t)i * p.ldres + j, t);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
+    if (p.c_f32) put8((float*)p.c + o, v); else put8((T*)p.c + o, v);
+  } else {
 #pragma unroll
-      for (int v = 0; v < 2; ++v) acc[u][v] = la_mma<T>(fa[u], fb[v], acc[u][v]);
-    __syncthreads();
+    for (int e = 0; e < 8; ++e) {
+      if (j + e >= p.n) continue;
+      float x = v[e], s;
+      if (p.bias) x += p.bias_f32 ? ((const float*)p.bias)[j + e] : (float)((const T*)p.bias)[j + e];
+      x = la_act(x, p.act, &s);
+      if (p.slope) ((S*)p.slope)[o + e] = (S)s;
+      if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j + e];
+      if (p.c_f32) ((float*)p.c)[o + e] = x; else ((T*)p.c)[o + e] = (T)x;
+    }
   }
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = i0 + wi + u * 16 + (lane >> 4) * 4 + r, j = j0 + wj + v * 16 + (lane & 15);
-        if (i < p.m && j < p.n) la_store<T>(p, i, j, acc[u][v][r]);
-      }
 }
 
-// dz = dy act'(z) and partial column sums of the unrounded dz: part[row chunk][n]
+// ---- tiles -------------------------------------------------------------------------------------------------------------
+// LDS-DMA through a buffer resource (16 bytes a lane; a lane whose offset is out of range gets zeros).  In asm, so that the
+// compiler does not wait for it before LDS reads: the ring below orders them with counted waits and barriers.  M0 is put back.
+typedef int la_srd_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ la_srd_t la_srd(const void* base) {
+  const unsigned long long b = (unsigned long long)base;
+  la_srd_t r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)(b & 0xFFFFFFFFull));
+  r[1] = __builtin_amdgcn_readfirstlane((int)(unsigned)((b >> 32) & 0xFFFFull));
+  r[2] = (int)0x80000000u;      // 2 GB of records: larger offsets are out of range
+  r[3] = 0x00020000;
+  return r;
+}
+__device__ __forceinline__ void la_dma16(la_srd_t srd, unsigned voff, unsigned lds_byte_off) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds_byte_off), "v"(voff), "s"(srd) : "memory");
+}
+__device__ __forceinline__ unsigned la_lds_addr(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)p;
+}
+template <int N> __device__ __forceinline__ void la_wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+typedef __attribute__((address_space(3))) bf16x4* la_tr_t;
+
+// One operand's tile: R rows (of C) x 128 bytes of k, in 16-byte pieces, stored so that the fragment reads below touch
+// every LDS bank once.
+//   k contiguous:   [row][8 pieces], piece p of row r in slot p ^ (r >> 1 & 7)
+//   row contiguous: [k][R elements]; the 32-byte (f32: 64-byte) column groups of k exchanged by the bits of k in which the
+//                   lanes of one read differ
+template <typename T, bool TR, int R, int NTH> struct LaTile {
+  static constexpr int EB = sizeof(T), PIECE = 16 / EB, KT = 128 / EB, LOADS = R * 8 / NTH, BYTES = R * 128, RB = R * EB;
+  unsigned voff[LOADS];
+  int kof[LOADS];
+  __device__ __forceinline__ void init(int tid, int row0, int rows, int64_t ld) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = i * NTH + tid;
+      if constexpr (!TR) {
+        const int r = q >> 3, pc = (q & 7) ^ ((r >> 1) & 7);
+        kof[i] = pc * PIECE;
+        voff[i] = row0 + r < rows ? (unsigned)(r * ld * EB) + pc * 16 : 0xFFFFFFFFu;
+      } else {
+        constexpr int PPR = RB / 16;
+        const int k = q / PPR, sl = q % PPR;
+        const int pc = EB == 2 ? ((((sl >> 1) ^ swz(k)) << 1) | (sl & 1)) : ((((sl >> 2) ^ swz(k)) << 2) | (sl & 3));
+        kof[i] = k;
+        voff[i] = row0 + pc * PIECE < rows ? (unsigned)(k * ld * EB) + pc * 16 : 0xFFFFFFFFu;
+      }
+    }
+  }
+  static __device__ __forceinline__ int swz(int k) { return EB == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3; }
+  // k0: first k of the tile; klimit: pieces at or beyond it come as zeros
+  __device__ __forceinline__ void load(int i, la_srd_t srd, unsigned lds, int wave, int k0, int klimit) const {
+    la_dma16(srd, k0 + kof[i] < klimit ? voff[i] : 0xFFFFFFFFu, lds + (i * NTH + wave * 64) * 16);
+  }
+  static __device__ __forceinline__ int64_t step(int64_t ld) { return TR ? KT * ld * EB : 128; }
+  static __device__ __forceinline__ u32x4 frag(const unsigned char* s, int tile, int ks, int lane) {
+    const int l16 = lane & 15, kg = lane >> 4;
+    if constexpr (!TR) {
+      const int r = tile * 16 + l16;
+      return *(const u32x4*)(s + r * 128 + (((ks * 4 + kg) ^ ((r >> 1) & 7)) << 4));
+    } else if constexpr (EB == 2) {
+      const int tq = l16 >> 2, tp = l16 & 3, k = ks * 32 + kg * 8 + tq;
+      const unsigned char* a = s + k * RB + ((tile ^ (tq | (kg & 1) << 2)) << 5) + tp * 8;
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_tr_t)a);
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_tr_t)(a + 4 * RB));
+      return __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    } else {
+      const unsigned* a = (const unsigned*)(s + (ks * 16 + kg * 4) * RB + ((tile ^ kg) << 6)) + l16;
+      return u32x4{a[0], a[RB / 4], a[2 * (RB / 4)], a[3 * (RB / 4)]};
+    }
+  }
+};
+
+__device__ __forceinline__ int la_xcd(int bid, int nblk) {      // blocks of one XCD (bid % 8) get one contiguous range of tiles
+  const int q = nblk >> 3, r = nblk & 7, x = bid & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
+}
+
+// WM x WN waves, each MT x NT products of 16 x 16; a ring of S tiles of 128 bytes of k; one barrier a tile
+template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(const GemmParams p) {
+  constexpr int NTH = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+  typedef LaTile<T, TA, BM, NTH> TileA;
+  typedef LaTile<T, TB, BN, NTH> TileB;
+  constexpr int STAGE = TileA::BYTES + TileB::BYTES, LOADS = TileA::LOADS + TileB::LOADS, KT = TileA::KT;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN, tiles = tm * tn;
+  int id = la_xcd(blockIdx.x, gridDim.x);
+  const int split = id / tiles;
+  id -= split * tiles;
+  // tiles in groups of 8 rows of tiles, so that the tiles an XCD works on at one time share rows and columns
+  const int group = id / (8 * tn), gm = tm - group * 8 < 8 ? tm - group * 8 : 8;
+  const int in = id - group * 8 * tn;
+  const int i0 = (group * 8 + in % gm) * BM, j0 = in / gm * BN;
+
+  TileA ta;
+  TileB tb;
+  ta.init(tid, i0, p.m, p.lda);
+  tb.init(tid, j0, p.n, p.ldb);
+  const int kt0 = split * p.ktiles, kt1 = min(kt0 + p.ktiles, (p.k + KT - 1) / KT);
+  const char* ga = (const char*)p.a + (TA ? (int64_t)i0 * sizeof(T) : (int64_t)i0 * p.lda * (int64_t)sizeof(T)) + kt0 * TileA::step(p.lda);
+  const char* gb = (const char*)p.b + (TB ? (int64_t)j0 * sizeof(T) : (int64_t)j0 * p.ldb * (int64_t)sizeof(T)) + kt0 * TileB::step(p.ldb);
+  const int klimit = min(p.k, kt1 * KT);
+  const unsigned lds0 = la_lds_addr(smem);
+  int kload = kt0 * KT, slot = 0;
+  auto issue = [&]() {
+    const la_srd_t sa = la_srd(ga), sb = la_srd(gb);
+    const unsigned base = lds0 + slot * STAGE;
+#pragma unroll
+    for (int i = 0; i < TileA::LOADS; ++i) ta.load(i, sa, base, wave, kload, klimit);
+#pragma unroll
+    for (int i = 0; i < TileB::LOADS; ++i) tb.load(i, sb, base + TileA::BYTES, wave, kload, klimit);
+    if (kload + KT < klimit) { ga += TileA::step(p.lda); gb += TileB::step(p.ldb); }      // past the end only zeros are asked for
+    kload += KT;
+    slot = slot + 1 == S ? 0 : slot + 1;
+  };
+  f32x4 acc[MT][NT] = {};
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue();
+  int cur = 0;
+  for (int kt = kt0; kt < kt1; ++kt) {
+    la_wait_barrier<(S - 2) * LOADS>();              // tile kt is in LDS, and nobody reads the slot that is filled next
+    issue();
+    const unsigned char *sa = smem + cur * STAGE, *sb = sa + TileA::BYTES;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u32x4 fa[MT], fb[NT];
+#pragma unroll
+      for (int u = 0; u < MT; ++u) fa[u] = TileA::frag(sa, wm * MT + u, ks, lane);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) fb[u] = TileB::frag(sb, wn * NT + u, ks, lane);
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+#pragma unroll
+        for (int v = 0; v < NT; ++v) acc[u][v] = la_mma<T>(fb[v], fa[u], acc[u][v]);
+    }
+    cur = cur + 1 == S ? 0 : cur + 1;
+  }
+  la_wait_barrier<0>();                              // the zeros asked for past the end have landed: LDS is free
+
+  // acc[u][v][r] of a lane: row 16 u + lane % 16, column 16 v + 4 (lane / 16) + r.  Through LDS (half of the wave's rows at a
+  // time), so that a lane finishes eight neighbouring columns and a row of the wave's tile leaves as one run of memory.
+  constexpr int LDW = 16 * NT + 4, HALF = MT / 2;
+  float* st = (float*)smem + wave * 16 * HALF * LDW;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int u = 0; u < HALF; ++u)
+#pragma unroll
+      for (int v = 0; v < NT; ++v) *(f32x4*)(st + (u * 16 + (lane & 15)) * LDW + v * 16 + (lane >> 4) * 4) = acc[h * HALF + u][v];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 1
+    for (int q = lane; q < 32 * NT * HALF; q += 64) {
+      const int r = q / (2 * NT), c = (q % (2 * NT)) * 8;
+      const int i = i0 + (wm * MT + h * HALF) * 16 + r, j = j0 + wn * NT * 16 + c;
+      float v[8];
+      *(f32x4*)v = *(const f32x4*)(st + r * LDW + c);
+      *(f32x4*)(v + 4) = *(const f32x4*)(st + r * LDW + c + 4);
+      if (i < p.m && j < p.n) {
+        if (p.part) put8(p.part + ((int64_t)split * p.m + i) * p.ldp + j, v);
+        else la_finish8<T>(p, i, j, v);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// sums of the splits in their order, and the epilogue
+template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmParams p) {
+  const int per = p.ldp / 8;
+  const int64_t q = blockIdx.x * (int64_t)256 + threadIdx.x;
+  if (q >= (int64_t)p.m * per) return;
+  const int i = (int)(q / per), j = (int)(q % per) * 8;
+  float v[8], t[8];
+  get8(p.part + (int64_t)i * p.ldp + j, v);
+  for (int s = 1; s < p.splits; ++s) {
+    get8(p.part + ((int64_t)s * p.m + i) * p.ldp + j, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  la_finish8<T>(p, i, j, v);
+}
+
+// [rows][cols] (row stride ld) into [rows][pitch], the padding zeroed; S -> T rounds (an f32 master weight for bf16 products)
+template <typename S, typename T>
+__global__ __launch_bounds__(256) void la_pack_kernel(const S* __restrict__ src, int64_t ld, T* __restrict__ dst, int64_t rows, int cols, int pitch) {
+  const int per = pitch / 8;
+  for (int64_t q = blockIdx.x * (int64_t)256 + threadIdx.x; q < rows * per; q += (int64_t)gridDim.x * 256) {
+    const int64_t r = q / per;
+    const int c = (int)(q % per) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)src[r * ld + c + e] : 0.f;
+    put8(dst + r * pitch + c, v);
+  }
+}
+
+// dz = dy slope (dz = dy without one) and partial column sums of the unrounded dz: part[row chunk][n]
 template <typename T>
-__global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
-                                                    float* __restrict__ part, int m, int n, int act, int rows_per) {
+__global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, const typename SlopeT<T>::type* __restrict__ slope, T* __restrict__ dz,
+                                                    float* __restrict__ part, int m, int n, int rows_per) {
   const int j = blockIdx.x * 256 + threadIdx.x;
   if (j >= n) return;
   const int r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < m ? r0 + rows_per : m;
@@ -118,8 +328,8 @@ __global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, co
   for (int r = r0; r < r1; ++r) {
     const int64_t o = (int64_t)r * n + j;
     float g = (float)dy[o];
-    if (act != VG_ACT_NONE) {
-      g *= la_slope((float)z[o], act);
+    if (slope) {
+      g *= (float)slope[o];
       dz[o] = (T)g;
     }
     s += g;
@@ -127,40 +337,140 @@ __global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, co
   if (part) part[(int64_t)blockIdx.y * n + j] = s;
 }
 
-static int la_gemm(const GemmParams& p, int dtype, hipStream_t st) {
-  const int64_t tiles = vg_ceil_div(p.n, 64) * vg_ceil_div(p.m, 64);
-  VG_REQUIRE(tiles < (1LL << 31), "linear_act: %d x %d outputs are too many for one launch", p.m, p.n);
-  const dim3 grid((unsigned)tiles);
-  if (dtype == VG_BF16) hipLaunchKernelGGL(gemm_any_kernel<bf16_t>, grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(gemm_any_kernel<float>, grid, dim3(256), 0, st, p);
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+// An operand as the tiles read it: the caller's matrix where it has 16-byte rows, otherwise a zero-padded copy.
+struct LaOperand {
+  const void* p;
+  int64_t ld, rows, cols;       // of the stored matrix
+  int src_f32;                  // f32 master weight of bf16 products
+};
+static size_t la_up(size_t n) { return (n + 255) / 256 * 256; }
+static int64_t la_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
+static bool la_direct(const LaOperand& o, int dtype) {
+  const int e = vg_elt_size(dtype);
+  return !(o.src_f32 && dtype == VG_BF16) && (uintptr_t)o.p % 16 == 0 && o.cols % (16 / e) == 0 && (o.ld * e) % 16 == 0 && o.ld * e < (1LL << 23);      // 255 rows within 2 GB
+}
+static size_t la_packed_bytes(const LaOperand& o, int dtype) { return la_up((size_t)o.rows * la_pitch(o.cols) * vg_elt_size(dtype)); }
+
+// which tiles, and how many ways the contraction is split
+struct LaPlan { int big, splits, ktiles; };
+static LaPlan la_plan(int64_t m, int64_t n, int64_t k, int dtype) {
+  const int64_t kt = vg_ceil_div(k * vg_elt_size(dtype), 128);
+  LaPlan p;
+  const int64_t t256 = vg_ceil_div(m, 256) * vg_ceil_div(n, 256), t128 = vg_ceil_div(m, 128) * vg_ceil_div(n, 128);
+  p.big = t256 >= 200;
+  const int64_t tiles = p.big ? t256 : t128, slots = p.big ? 256 : 512;
+  int64_t s = 1;
+  if (tiles * 2 <= slots) {
+    s = slots / tiles;
+    if (s > kt / 4) s = kt / 4;                      // at least 4 tiles of k a split
+    if (s > 32) s = 32;
+    if (s < 1) s = 1;
+  }
+  p.ktiles = (int)vg_ceil_div(kt, s);
+  p.splits = (int)vg_ceil_div(kt, p.ktiles);
+  return p;
+}
+static size_t la_part_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
+  const LaPlan pl = la_plan(m, n, k, dtype);
+  return pl.splits > 1 ? la_up((size_t)pl.splits * m * la_pitch(n) * sizeof(float)) : 0;
+}
+static size_t la_ws(int64_t m, int64_t n, int64_t k, int dtype, const LaOperand& a, const LaOperand& b) {
+  return la_part_bytes(m, n, k, dtype) + (la_direct(a, dtype) ? 0 : la_packed_bytes(a, dtype)) + (la_direct(b, dtype) ? 0 : la_packed_bytes(b, dtype));
+}
+
+template <typename S, typename T> static void la_pack_launch(const LaOperand& o, void* dst, hipStream_t st) {
+  const int pitch = (int)la_pitch(o.cols);
+  int64_t blocks = vg_ceil_div(o.rows * (pitch / 8), 256);
+  if (blocks > 8192) blocks = 8192;
+  hipLaunchKernelGGL((la_pack_kernel<S, T>), dim3((unsigned)blocks), dim3(256), 0, st, (const S*)o.p, o.ld, (T*)dst, o.rows, (int)o.cols, pitch);
+}
+static char* la_pack(LaOperand* o, int dtype, char* ws, hipStream_t st) {
+  if (la_direct(*o, dtype)) return ws;
+  if (dtype == VG_F32) la_pack_launch<float, float>(*o, ws, st);
+  else if (o->src_f32) la_pack_launch<float, bf16_t>(*o, ws, st);
+  else la_pack_launch<bf16_t, bf16_t>(*o, ws, st);
+  const size_t n = la_packed_bytes(*o, dtype);
+  o->p = ws;
+  o->ld = la_pitch(o->cols);
+  return ws + n;
+}
+
+template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S> static int la_tile_launch(const GemmParams& p, hipStream_t st) {
+  constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
+  const int ring = S * (BM + BN) * 128, out = WM * WN * 8 * MT * (16 * NT + 4) * 4, lds = ring > out ? ring : out;
+  void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S>;
+  VG_HIP(vg_lds_attr((const void*)kernel, lds));
+  const int64_t blocks = vg_ceil_div(p.m, BM) * vg_ceil_div(p.n, BN) * p.splits;
+  VG_REQUIRE(blocks < (1LL << 31), "linear_act: %d x %d outputs are too many for one launch", p.m, p.n);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WM * WN), lds, st, p);
   VG_LAUNCH_CHECK();
   return VG_OK;
+}
+template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int dtype, char* ws, hipStream_t st) {
+  const LaPlan pl = la_plan(p.m, p.n, p.k, dtype);
+  p.splits = pl.splits;
+  p.ktiles = pl.ktiles;
+  p.ldp = (int)la_pitch(p.n);
+  p.part = pl.splits > 1 ? (float*)ws : nullptr;
+  const int rc = pl.big ? la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2>(p, st) : la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);
+  if (rc) return rc;
+  if (pl.splits > 1) {
+    hipLaunchKernelGGL(gemm_join_kernel<T>, dim3((unsigned)vg_ceil_div((int64_t)p.m * (p.ldp / 8), 256)), dim3(256), 0, st, p);
+    VG_LAUNCH_CHECK();
+  }
+  return VG_OK;
+}
+// C [m][n] = A B over k; a is stored [m][k] (ta: [k][m]), b [n][k] (tb: [k][n])
+static int la_gemm(GemmParams p, LaOperand a, bool ta, LaOperand b, bool tb, int dtype, void* ws, hipStream_t st) {
+  VG_REQUIRE((uintptr_t)ws % 256 == 0 && (ws || la_ws(p.m, p.n, p.k, dtype, a, b) == 0), "linear_act: needs a workspace, aligned to 256 bytes");
+  const int e = vg_elt_size(dtype);
+  char* w = la_pack(&a, dtype, (char*)ws, st);
+  w = la_pack(&b, dtype, w, st);
+  VG_LAUNCH_CHECK();
+  p.a = a.p; p.lda = a.ld; p.b = b.p; p.ldb = b.ld;
+  auto al = [](const void* q) { return (uintptr_t)q % 16 == 0; };
+  p.vec = p.n % 8 == 0 && al(p.c) && al(p.slope) && al(p.bias) && (!p.res || (al(p.res) && (p.ldres * e) % 16 == 0));
+  if (dtype == VG_BF16)
+    return ta ? la_gemm_t<bf16_t, true, true>(p, dtype, w, st) : tb ? la_gemm_t<bf16_t, false, true>(p, dtype, w, st) : la_gemm_t<bf16_t, false, false>(p, dtype, w, st);
+  return ta ? la_gemm_t<float, true, true>(p, dtype, w, st) : tb ? la_gemm_t<float, false, true>(p, dtype, w, st) : la_gemm_t<float, false, false>(p, dtype, w, st);
 }
 
 static int la_check(const char* what, int64_t m, int64_t n, int64_t k, int act, int dtype) {
   VG_REQUIRE(dtype == VG_F32 || dtype == VG_BF16, "%s: dtype %d", what, dtype);
-  VG_REQUIRE(m >= 1 && n >= 1 && k >= 1 && m < (1LL << 30) && n < (1LL << 22) && k < (1LL << 30), "%s: %ld x %ld x %ld", what, (long)m, (long)n, (long)k);
+  VG_REQUIRE(m >= 1 && n >= 1 && k >= 1 && m < (1LL << 30) && n < (1LL << 20) && k < (1LL << 20), "%s: %ld x %ld x %ld", what, (long)m, (long)n, (long)k);
   VG_REQUIRE(act >= VG_ACT_NONE && act <= VG_ACT_SILU, "%s: activation %d", what, act);
   return VG_OK;
 }
+static int la_weight(const char* what, int w_dtype, int dtype) {
+  VG_REQUIRE(w_dtype == dtype || w_dtype == VG_F32, "%s: weight dtype %d for dtype %d", what, w_dtype, dtype);
+  return VG_OK;
+}
 
-extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, const void* bias, int bias_dtype, const void* res,
-                                 int64_t ldres, void* y, void* z, int64_t m, int64_t n, int64_t k, int act, int dtype, void* stream) {
+extern "C" size_t vg_linear_act_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype) {
+  return la_ws(m, n, k, dtype, {x, ldx, m, k, 0}, {w, k, n, k, w_dtype == VG_F32});
+}
+extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int w_dtype, const void* bias, int bias_dtype, const void* res,
+                                 int64_t ldres, void* y, void* slope, void* ws, int64_t m, int64_t n, int64_t k, int act, int dtype,
+                                 void* stream) {
   if (int rc = la_check("linear_act_fwd", m, n, k, act, dtype)) return rc;
+  if (int rc = la_weight("linear_act_fwd", w_dtype, dtype)) return rc;
   VG_REQUIRE(x && w && y && ldx >= k && (!res || ldres >= n), "linear_act_fwd: null pointer or a short row stride");
-  GemmParams p = {x, w, ldx, 1, k, 1, (int)m, (int)n, (int)k, y, n, 0, bias, bias_dtype == VG_F32, res, ldres, z, act};
-  return la_gemm(p, dtype, (hipStream_t)stream);
+  GemmParams p = {};
+  p.m = (int)m; p.n = (int)n; p.k = (int)k;
+  p.c = y; p.bias = bias; p.bias_f32 = bias_dtype == VG_F32; p.res = res; p.ldres = ldres; p.slope = act == VG_ACT_NONE ? nullptr : slope; p.act = act;
+  return la_gemm(p, {x, ldx, m, k, 0}, false, {w, k, n, k, w_dtype == VG_F32}, false, dtype, ws, (hipStream_t)stream);
 }
 
 static const int LA_DZ_PARTS = 256;
 extern "C" size_t vg_linear_act_dz_ws_bytes(int64_t m, int64_t n) {
   return (size_t)(m < LA_DZ_PARTS ? m : LA_DZ_PARTS) * (size_t)n * sizeof(float);
 }
-extern "C" int vg_linear_act_dz(const void* dy, const void* z, void* dz, void* db, int bias_dtype, void* ws, int64_t m, int64_t n, int act,
+extern "C" int vg_linear_act_dz(const void* dy, const void* slope, void* dz, void* db, int bias_dtype, void* ws, int64_t m, int64_t n,
                                 int dtype, void* stream) {
-  if (int rc = la_check("linear_act_dz", m, n, 1, act, dtype)) return rc;
-  VG_REQUIRE(dy && (act == VG_ACT_NONE || (z && dz)) && (!db || ws), "linear_act_dz: null pointer");
-  if (act == VG_ACT_NONE && !db) return VG_OK;
+  if (int rc = la_check("linear_act_dz", m, n, 1, VG_ACT_NONE, dtype)) return rc;
+  VG_REQUIRE(dy && (!slope || dz) && (slope || db) && (!db || ws), "linear_act_dz: null pointer");
   hipStream_t st = (hipStream_t)stream;
   int parts = (int)(m < LA_DZ_PARTS ? m : LA_DZ_PARTS);
   const int per = (int)vg_ceil_div(m, parts);
@@ -168,24 +478,37 @@ extern "C" int vg_linear_act_dz(const void* dy, const void* z, void* dz, void* d
   const dim3 grid((unsigned)vg_ceil_div(n, 256), (unsigned)parts);
   float* part = db ? (float*)ws : nullptr;
   if (dtype == VG_BF16)
-    hipLaunchKernelGGL(la_dz_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)dy, (const bf16_t*)z, (bf16_t*)dz, part, (int)m, (int)n, act, per);
-  else hipLaunchKernelGGL(la_dz_kernel<float>, grid, dim3(256), 0, st, (const float*)dy, (const float*)z, (float*)dz, part, (int)m, (int)n, act, per);
+    hipLaunchKernelGGL(la_dz_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)dy, (const f16_t*)slope, (bf16_t*)dz, part, (int)m, (int)n, per);
+  else hipLaunchKernelGGL(la_dz_kernel<float>, grid, dim3(256), 0, st, (const float*)dy, (const float*)slope, (float*)dz, part, (int)m, (int)n, per);
   VG_LAUNCH_CHECK();
   if (db) return vg_fold_cols(part, parts, n, db, n, nullptr, bias_dtype, st);
   return VG_OK;
 }
 
-extern "C" int vg_linear_act_dgrad(const void* dz, const void* w, void* dx, int64_t m, int64_t n, int64_t k, int dtype, void* stream) {
+extern "C" size_t vg_linear_act_dgrad_ws_bytes(const void* dz, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype) {
+  return la_ws(m, k, n, dtype, {dz, n, m, n, 0}, {w, k, n, k, w_dtype == VG_F32});
+}
+extern "C" int vg_linear_act_dgrad(const void* dz, const void* w, int w_dtype, void* dx, void* ws, int64_t m, int64_t n, int64_t k, int dtype,
+                                   void* stream) {
   if (int rc = la_check("linear_act_dgrad", m, n, k, VG_ACT_NONE, dtype)) return rc;
-  VG_REQUIRE(k < (1LL << 22) && dz && w && dx, "linear_act_dgrad: null pointer, or too wide");
-  GemmParams p = {dz, w, n, 1, 1, k, (int)m, (int)k, (int)n, dx, k, 0, nullptr, 0, nullptr, 0, nullptr, VG_ACT_NONE};
-  return la_gemm(p, dtype, (hipStream_t)stream);
+  if (int rc = la_weight("linear_act_dgrad", w_dtype, dtype)) return rc;
+  VG_REQUIRE(dz && w && dx, "linear_act_dgrad: null pointer");
+  GemmParams p = {};
+  p.m = (int)m; p.n = (int)k; p.k = (int)n;
+  p.c = dx;
+  return la_gemm(p, {dz, n, m, n, 0}, false, {w, k, n, k, w_dtype == VG_F32}, true, dtype, ws, (hipStream_t)stream);
 }
 
-extern "C" int vg_linear_act_wgrad(const void* dz, const void* x, int64_t ldx, void* dw, int dw_dtype, int64_t m, int64_t n, int64_t k,
+extern "C" size_t vg_linear_act_wgrad_ws_bytes(const void* dz, const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k, int dtype) {
+  return la_ws(n, k, m, dtype, {dz, n, m, n, 0}, {x, ldx, m, k, 0});
+}
+extern "C" int vg_linear_act_wgrad(const void* dz, const void* x, int64_t ldx, void* dw, int dw_dtype, void* ws, int64_t m, int64_t n, int64_t k,
                                    int dtype, void* stream) {
   if (int rc = la_check("linear_act_wgrad", m, n, k, VG_ACT_NONE, dtype)) return rc;
-  VG_REQUIRE(k < (1LL << 22) && dz && x && dw && ldx >= k, "linear_act_wgrad: null pointer, a short row stride, or too wide");
-  GemmParams p = {dz, x, 1, n, 1, ldx, (int)n, (int)k, (int)m, dw, k, dw_dtype == VG_F32, nullptr, 0, nullptr, 0, nullptr, VG_ACT_NONE};
-  return la_gemm(p, dtype, (hipStream_t)stream);
+  if (int rc = la_weight("linear_act_wgrad", dw_dtype, dtype)) return rc;
+  VG_REQUIRE(dz && x && dw && ldx >= k, "linear_act_wgrad: null pointer or a short row stride");
+  GemmParams p = {};
+  p.m = (int)n; p.n = (int)k; p.k = (int)m;
+  p.c = dw; p.c_f32 = dw_dtype == VG_F32;
+  return la_gemm(p, {dz, n, m, n, 0}, true, {x, ldx, m, k, 0}, true, dtype, ws, (hipStream_t)stream);
 }

@@ -123,11 +123,14 @@ SIGNATURES = {
     "vg_layer_norm_fwd": (_I, [_P, _L, _P, _P, _P, _L, _P, _L, _I, _I, _F, _I, _P]),
     "vg_layer_norm_bwd_ws_bytes": (C.c_size_t, [_L, _I]),
     "vg_layer_norm_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _P]),
-    "vg_linear_act_fwd": (_I, [_P, _L, _P, _P, _I, _P, _L, _P, _P, _L, _L, _L, _I, _I, _P]),
+    "vg_linear_act_fwd_ws_bytes": (C.c_size_t, [_P, _L, _P, _I, _L, _L, _L, _I]),
+    "vg_linear_act_fwd": (_I, [_P, _L, _P, _I, _P, _I, _P, _L, _P, _P, _P, _L, _L, _L, _I, _I, _P]),
     "vg_linear_act_dz_ws_bytes": (C.c_size_t, [_L, _L]),
-    "vg_linear_act_dz": (_I, [_P, _P, _P, _P, _I, _P, _L, _L, _I, _I, _P]),
-    "vg_linear_act_dgrad": (_I, [_P, _P, _P, _L, _L, _L, _I, _P]),
-    "vg_linear_act_wgrad": (_I, [_P, _P, _L, _P, _I, _L, _L, _L, _I, _P]),
+    "vg_linear_act_dz": (_I, [_P, _P, _P, _P, _I, _P, _L, _L, _I, _P]),
+    "vg_linear_act_dgrad_ws_bytes": (C.c_size_t, [_P, _P, _I, _L, _L, _L, _I]),
+    "vg_linear_act_dgrad": (_I, [_P, _P, _I, _P, _P, _L, _L, _L, _I, _P]),
+    "vg_linear_act_wgrad_ws_bytes": (C.c_size_t, [_P, _P, _L, _L, _L, _L, _I]),
+    "vg_linear_act_wgrad": (_I, [_P, _P, _L, _P, _I, _P, _L, _L, _L, _I, _P]),
     "vg_token_logprobs_ws_bytes": (C.c_size_t, [_L, _I, _I]),
     "vg_token_logprobs_fwd": (_I, [_P, _L, _P, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P]),
     "vg_token_logprobs_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),

@@ -1358,62 +1358,67 @@ def layer_norm(x, weight, bias, eps: float = 1e-5, c: Optional[int] = None):
     return LayerNormFn.apply(x, weight, bias, float(eps), c)
 
 
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 class LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
         lib = L.load()
-        dt = x.dtype
+        dt, code, wcode = x.dtype, L.vg_dtype(x.dtype), L.vg_dtype(weight.dtype)
         n, k = weight.shape
         xr, ldx = _rows_of(x)
         m = xr.shape[0]
         y = torch.empty(*x.shape[:-1], n, dtype=dt, device=x.device)
-        w = weight.to(dt).contiguous()
+        w = weight.contiguous()
         b = None if bias is None else bias.contiguous()
-        z = None
+        slope = None
         if m:
             rr, ldr = _rows_of(residual) if residual is not None else (None, 0)
             if act != L.ACT_NONE and any(ctx.needs_input_grad[:3]):
-                z = torch.empty(m, n, dtype=dt, device=x.device)
+                slope = torch.empty(m, n, dtype=torch.float16 if dt == torch.bfloat16 else torch.float32, device=x.device)
+            ws = _workspace(lib.vg_linear_act_fwd_ws_bytes(xr.data_ptr(), ldx, w.data_ptr(), wcode, m, n, k, code), x.device)
             with _on_device("linear_act", x):
-                L.check(lib.vg_linear_act_fwd(xr.data_ptr(), ldx, w.data_ptr(), L.ptr(b), 0 if b is None else L.vg_dtype(b.dtype),
-                                              L.ptr(rr), ldr, y.data_ptr(), L.ptr(z), m, n, k, act, L.vg_dtype(dt), L.stream()),
+                L.check(lib.vg_linear_act_fwd(xr.data_ptr(), ldx, w.data_ptr(), wcode, L.ptr(b), 0 if b is None else L.vg_dtype(b.dtype),
+                                              L.ptr(rr), ldr, y.data_ptr(), L.ptr(slope), L.ptr(ws), m, n, k, act, code, L.stream()),
                         "linear_act_fwd")
-        ctx.save_for_backward(x, w, z)
-        ctx.act = act
-        ctx.wdt, ctx.bdt = weight.dtype, None if bias is None else bias.dtype
+        ctx.save_for_backward(x, w, slope)
+        ctx.bdt = None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        x, w, z = ctx.saved_tensors
+        x, w, slope = ctx.saved_tensors
         lib = L.load()
-        dt, act = x.dtype, ctx.act
-        code = L.vg_dtype(dt)
+        dt, dev = x.dtype, x.device
+        code, wcode = L.vg_dtype(dt), L.vg_dtype(w.dtype)
         n, k = w.shape
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
         xr, ldx = _rows_of(x)
         m = xr.shape[0]
-        dx = torch.empty(x.shape, dtype=dt, device=x.device) if need_x else None
-        dw = torch.empty(n, k, dtype=ctx.wdt, device=x.device) if need_w else None
-        db = torch.empty(n, dtype=ctx.bdt, device=x.device) if need_b else None
+        dx = torch.empty(x.shape, dtype=dt, device=dev) if need_x else None
+        dw = torch.empty(n, k, dtype=w.dtype, device=dev) if need_w else None
+        db = torch.empty(n, dtype=ctx.bdt, device=dev) if need_b else None
         if m == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, gy if need_r else None
         g = gy.reshape(m, n).contiguous()
         with _on_device("linear_act", x):
             dz = g
-            if need_b or (act != L.ACT_NONE and (need_x or need_w)):
-                ws = None
-                if need_b:
-                    ws = torch.empty(lib.vg_linear_act_dz_ws_bytes(m, n), dtype=torch.uint8, device=x.device)
-                if act != L.ACT_NONE:
-                    dz = torch.empty(m, n, dtype=dt, device=x.device)
-                L.check(lib.vg_linear_act_dz(g.data_ptr(), L.ptr(z), dz.data_ptr(), L.ptr(db), 0 if db is None else L.vg_dtype(ctx.bdt),
-                                             L.ptr(ws), m, n, act, code, L.stream()), "linear_act_dz")
+            if need_b or (slope is not None and (need_x or need_w)):
+                ws = _workspace(lib.vg_linear_act_dz_ws_bytes(m, n) if need_b else 0, dev)
+                if slope is not None:
+                    dz = torch.empty(m, n, dtype=dt, device=dev)
+                L.check(lib.vg_linear_act_dz(g.data_ptr(), L.ptr(slope), dz.data_ptr(), L.ptr(db), 0 if db is None else L.vg_dtype(ctx.bdt),
+                                             L.ptr(ws), m, n, code, L.stream()), "linear_act_dz")
             if need_x:
-                L.check(lib.vg_linear_act_dgrad(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), m, n, k, code, L.stream()), "linear_act_dgrad")
+                ws = _workspace(lib.vg_linear_act_dgrad_ws_bytes(dz.data_ptr(), w.data_ptr(), wcode, m, n, k, code), dev)
+                L.check(lib.vg_linear_act_dgrad(dz.data_ptr(), w.data_ptr(), wcode, dx.data_ptr(), L.ptr(ws), m, n, k, code, L.stream()),
+                        "linear_act_dgrad")
             if need_w:
-                L.check(lib.vg_linear_act_wgrad(dz.data_ptr(), xr.data_ptr(), ldx, dw.data_ptr(), L.vg_dtype(ctx.wdt), m, n, k, code,
+                ws = _workspace(lib.vg_linear_act_wgrad_ws_bytes(dz.data_ptr(), xr.data_ptr(), ldx, m, n, k, code), dev)
+                L.check(lib.vg_linear_act_wgrad(dz.data_ptr(), xr.data_ptr(), ldx, dw.data_ptr(), wcode, L.ptr(ws), m, n, k, code,
                                                 L.stream()), "linear_act_wgrad")
         return dx, dw, db, None, gy if need_r else None
 
