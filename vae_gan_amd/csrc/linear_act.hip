@@ -11,19 +11,23 @@
 typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef _Float16 f16_t;
 
-// act(z) and act'(z), sharing the exponential
+// act(z) and act'(z), sharing the exponential.  Phi(-|z|) of GELU is half of Abramowitz & Stegun 7.1.26 (erfc to 1.5e-7, from
+// the same e^(-z^2/2) as the density): a library erf costs four times the instructions, and 67 M of them took as long as the
+// product of 16384 x 1024 x 4096 itself.
 __device__ __forceinline__ float la_act(float z, int act, float* slope) {
   float y = z, s = 1.f;
   switch (act) {
     case VG_ACT_LRELU: s = z > 0.f ? 1.f : VG_LRELU_SLOPE; y = z * s; break;
-    case VG_ACT_SIGMOID: y = 1.f / (1.f + __expf(-z)); s = y * (1.f - y); break;
+    case VG_ACT_SIGMOID: y = __builtin_amdgcn_rcpf(1.f + __expf(-z)); s = y * (1.f - y); break;
     case VG_ACT_GELU: {
-      const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+      const float e = __expf(-0.5f * z * z), t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * fabsf(z));
+      const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+      const float phi = z < 0.f ? q : 1.f - q;
       y = z * phi;
-      s = phi + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+      s = phi + z * e * 0.39894228040143268f;
       break;
     }
-    case VG_ACT_SILU: { const float p = 1.f / (1.f + __expf(-z)); y = z * p; s = p * (1.f + z * (1.f - p)); break; }
+    case VG_ACT_SILU: { const float p = __builtin_amdgcn_rcpf(1.f + __expf(-z)); y = z * p; s = p * (1.f + z * (1.f - p)); break; }
     default: break;
   }
   *slope = s;
@@ -144,6 +148,7 @@ typedef __attribute__((address_space(3))) bf16x4* la_tr_t;
 //                   lanes of one read differ
 template <typename T, bool TR, int R, int NTH> struct LaTile {
   static constexpr int EB = sizeof(T), PIECE = 16 / EB, KT = 128 / EB, LOADS = R * 8 / NTH, BYTES = R * 128, RB = R * EB;
+  static constexpr int FRAG_READS = TR ? (EB == 2 ? 2 : 4) : 1;
   unsigned voff[LOADS];
   int kof[LOADS];
   __device__ __forceinline__ void init(int tid, int row0, int rows, int64_t ld) {
@@ -233,26 +238,44 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(const GemmParam
     slot = slot + 1 == S ? 0 : slot + 1;
   };
   f32x4 acc[MT][NT] = {};
+  // Two sets of fragments: while the products of one half of a tile run, the other half (or the next tile's first half) is
+  // read from LDS.  Without that the eight waves read together and multiply together, and each unit idles half the time.
+  u32x4 fa[2][MT], fb[2][NT];
+  auto read = [&](int set, const unsigned char* s, int ks) {
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) issue();
+    for (int u = 0; u < MT; ++u) fa[set][u] = TileA::frag(s, wm * MT + u, ks, lane);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) fb[set][u] = TileB::frag(s + TileA::BYTES, wn * NT + u, ks, lane);
+  };
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int v = 0; v < NT; ++v) acc[u][v] = la_mma<T>(fb[set][v], fa[set][u], acc[u][v]);
+  };
+  constexpr int READS = MT * TileA::FRAG_READS + NT * TileB::FRAG_READS, PRODUCTS = MT * NT * (sizeof(T) == 2 ? 1 : 4);
+  auto interleave = [&]() {                          // one LDS read every few products
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS, 0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) issue();
+  la_wait_barrier<(S - 1) * LOADS>();
+  read(0, smem, 0);
   int cur = 0;
   for (int kt = kt0; kt < kt1; ++kt) {
-    la_wait_barrier<(S - 2) * LOADS>();              // tile kt is in LDS, and nobody reads the slot that is filled next
-    issue();
-    const unsigned char *sa = smem + cur * STAGE, *sb = sa + TileA::BYTES;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4 fa[MT], fb[NT];
-#pragma unroll
-      for (int u = 0; u < MT; ++u) fa[u] = TileA::frag(sa, wm * MT + u, ks, lane);
-#pragma unroll
-      for (int u = 0; u < NT; ++u) fb[u] = TileB::frag(sb, wn * NT + u, ks, lane);
-#pragma unroll
-      for (int u = 0; u < MT; ++u)
-#pragma unroll
-        for (int v = 0; v < NT; ++v) acc[u][v] = la_mma<T>(fb[v], fa[u], acc[u][v]);
-    }
+    read(1, smem + cur * STAGE, 1);
+    multiply(0);
+    interleave();
+    la_wait_barrier<(S - 2) * LOADS>();              // tile kt + 1 is in LDS, and everyone has read tile kt
+    issue();                                         // tile kt + S takes its place
     cur = cur + 1 == S ? 0 : cur + 1;
+    read(0, smem + cur * STAGE, 0);                  // past the last tile: zeros
+    multiply(1);
+    interleave();
   }
   la_wait_barrier<0>();                              // the zeros asked for past the end have landed: LDS is free
 
@@ -359,7 +382,7 @@ static LaPlan la_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   const int64_t kt = vg_ceil_div(k * vg_elt_size(dtype), 128);
   LaPlan p;
   const int64_t t256 = vg_ceil_div(m, 256) * vg_ceil_div(n, 256), t128 = vg_ceil_div(m, 128) * vg_ceil_div(n, 128);
-  p.big = t256 >= 200;
+  p.big = dtype == VG_BF16 && t256 >= 200;
   const int64_t tiles = p.big ? t256 : t128, slots = p.big ? 256 : 512;
   int64_t s = 1;
   if (tiles * 2 <= slots) {
@@ -414,7 +437,9 @@ template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int d
   p.ktiles = pl.ktiles;
   p.ldp = (int)la_pitch(p.n);
   p.part = pl.splits > 1 ? (float*)ws : nullptr;
-  const int rc = pl.big ? la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2>(p, st) : la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);
+  int rc;
+  if constexpr (sizeof(T) == 2) rc = pl.big ? la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2>(p, st) : la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);
+  else rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);       // bound by the f32 matrix rate at either size
   if (rc) return rc;
   if (pl.splits > 1) {
     hipLaunchKernelGGL(gemm_join_kernel<T>, dim3((unsigned)vg_ceil_div((int64_t)p.m * (p.ldp / 8), 256)), dim3(256), 0, st, p);
