@@ -141,13 +141,14 @@ template <int N> __device__ __forceinline__ void la_wait_barrier() {
 }
 typedef __attribute__((address_space(3))) bf16x4* la_tr_t;
 
-// One operand's tile: R rows (of C) x 128 bytes of k, in 16-byte pieces, stored so that the fragment reads below touch
-// every LDS bank once.
-//   k contiguous:   [row][8 pieces], piece p of row r in slot p ^ (r >> 1 & 7)
+// One operand's tile: R rows (of C) x KB bytes of k (64 or 128), in 16-byte pieces, stored so that the fragment reads below
+// touch every LDS bank once.
+//   k contiguous:   [row][KB / 16 pieces], piece p of row r in slot p ^ (r >> 1 & 7) (KB 64: p ^ (r >> 2 & 3))
 //   row contiguous: [k][R elements]; the 32-byte (f32: 64-byte) column groups of k exchanged by the bits of k in which the
 //                   lanes of one read differ
-template <typename T, bool TR, int R, int NTH> struct LaTile {
-  static constexpr int EB = sizeof(T), PIECE = 16 / EB, KT = 128 / EB, LOADS = R * 8 / NTH, BYTES = R * 128, RB = R * EB;
+template <typename T, bool TR, int R, int NTH, int KB> struct LaTile {
+  static constexpr int EB = sizeof(T), PIECE = 16 / EB, KT = KB / EB, LOADS = R * (KB / 16) / NTH, BYTES = R * KB, RB = R * EB;
+  static __device__ __forceinline__ int turn(int r) { return KB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
   static constexpr int FRAG_READS = TR ? (EB == 2 ? 2 : 4) : 1;
   unsigned voff[LOADS];
   int kof[LOADS];
@@ -156,7 +157,7 @@ template <typename T, bool TR, int R, int NTH> struct LaTile {
     for (int i = 0; i < LOADS; ++i) {
       const int q = i * NTH + tid;
       if constexpr (!TR) {
-        const int r = q >> 3, pc = (q & 7) ^ ((r >> 1) & 7);
+        const int r = q / (KB / 16), pc = (q % (KB / 16)) ^ turn(r);
         kof[i] = pc * PIECE;
         voff[i] = row0 + r < rows ? (unsigned)(r * ld * EB) + pc * 16 : 0xFFFFFFFFu;
       } else {
@@ -173,12 +174,12 @@ template <typename T, bool TR, int R, int NTH> struct LaTile {
   __device__ __forceinline__ void load(int i, la_srd_t srd, unsigned lds, int wave, int k0, int klimit) const {
     la_dma16(srd, k0 + kof[i] < klimit ? voff[i] : 0xFFFFFFFFu, lds + (i * NTH + wave * 64) * 16);
   }
-  static __device__ __forceinline__ int64_t step(int64_t ld) { return TR ? KT * ld * EB : 128; }
+  static __device__ __forceinline__ int64_t step(int64_t ld) { return TR ? KT * ld * EB : KB; }
   static __device__ __forceinline__ u32x4 frag(const unsigned char* s, int tile, int ks, int lane) {
     const int l16 = lane & 15, kg = lane >> 4;
     if constexpr (!TR) {
       const int r = tile * 16 + l16;
-      return *(const u32x4*)(s + r * 128 + (((ks * 4 + kg) ^ ((r >> 1) & 7)) << 4));
+      return *(const u32x4*)(s + r * KB + (((ks * 4 + kg) ^ turn(r)) << 4));
     } else if constexpr (EB == 2) {
       const int tq = l16 >> 2, tp = l16 & 3, k = ks * 32 + kg * 8 + tq;
       const unsigned char* a = s + k * RB + ((tile ^ (tq | (kg & 1) << 2)) << 5) + tp * 8;
@@ -197,12 +198,12 @@ __device__ __forceinline__ int la_xcd(int bid, int nblk) {      // blocks of one
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
 }
 
-// WM x WN waves, each MT x NT products of 16 x 16; a ring of S tiles of 128 bytes of k; one barrier a tile
-template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(const GemmParams p) {
+// WM x WN waves, each MT x NT products of 16 x 16; a ring of S tiles of KB bytes of k; one barrier a tile
+template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S, int KB>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmParams p) {
   constexpr int NTH = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
-  typedef LaTile<T, TA, BM, NTH> TileA;
-  typedef LaTile<T, TB, BN, NTH> TileB;
+  typedef LaTile<T, TA, BM, NTH, KB> TileA;
+  typedef LaTile<T, TB, BN, NTH, KB> TileB;
   constexpr int STAGE = TileA::BYTES + TileB::BYTES, LOADS = TileA::LOADS + TileB::LOADS, KT = TileA::KT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -266,14 +267,18 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(const GemmParam
   la_wait_barrier<(S - 1) * LOADS>();
   read(0, smem, 0);
   int cur = 0;
-  for (int kt = kt0; kt < kt1; ++kt) {
-    read(1, smem + cur * STAGE, 1);
-    multiply(0);
-    interleave();
-    la_wait_barrier<(S - 2) * LOADS>();              // tile kt + 1 is in LDS, and everyone has read tile kt
+  auto next = [&]() {
+    la_wait_barrier<(S - 2) * LOADS>();              // the next tile is in LDS, and everyone has read this one
     issue();                                         // tile kt + S takes its place
     cur = cur + 1 == S ? 0 : cur + 1;
-    read(0, smem + cur * STAGE, 0);                  // past the last tile: zeros
+  };
+  for (int kt = kt0; kt < kt1; kt += KB == 128 ? 1 : 2) {      // past the last tile: zeros
+    if constexpr (KB == 64) next();
+    read(1, smem + cur * STAGE, KB == 64 ? 0 : 1);
+    multiply(0);
+    interleave();
+    next();
+    read(0, smem + cur * STAGE, 0);
     multiply(1);
     interleave();
   }
@@ -420,10 +425,11 @@ static char* la_pack(LaOperand* o, int dtype, char* ws, hipStream_t st) {
   return ws + n;
 }
 
-template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S> static int la_tile_launch(const GemmParams& p, hipStream_t st) {
+template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S, int KB> static int la_tile_launch(GemmParams p, hipStream_t st) {
+  p.ktiles *= 128 / KB;                              // the plan counts 128 bytes of k
   constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
-  const int ring = S * (BM + BN) * 128, out = WM * WN * 8 * MT * (16 * NT + 4) * 4, lds = ring > out ? ring : out;
-  void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S>;
+  const int ring = S * (BM + BN) * KB, out = WM * WN * 8 * MT * (16 * NT + 4) * 4, lds = ring > out ? ring : out;
+  void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S, KB>;
   VG_HIP(vg_lds_attr((const void*)kernel, lds));
   const int64_t blocks = vg_ceil_div(p.m, BM) * vg_ceil_div(p.n, BN) * p.splits;
   VG_REQUIRE(blocks < (1LL << 31), "linear_act: %d x %d outputs are too many for one launch", p.m, p.n);
@@ -438,8 +444,8 @@ template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int d
   p.ldp = (int)la_pitch(p.n);
   p.part = pl.splits > 1 ? (float*)ws : nullptr;
   int rc;
-  if constexpr (sizeof(T) == 2) rc = pl.big ? la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2>(p, st) : la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);
-  else rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);       // bound by the f32 matrix rate at either size
+  if constexpr (sizeof(T) == 2) rc = pl.big ? la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2, 128>(p, st) : la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2, 128>(p, st);
+  else rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2, 128>(p, st);       // bound by the f32 matrix rate at either size
   if (rc) return rc;
   if (pl.splits > 1) {
     hipLaunchKernelGGL(gemm_join_kernel<T>, dim3((unsigned)vg_ceil_div((int64_t)p.m * (p.ldp / 8), 256)), dim3(256), 0, st, p);
