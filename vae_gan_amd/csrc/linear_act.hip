@@ -14,24 +14,36 @@ typedef _Float16 f16_t;
 // act(z) and act'(z), sharing the exponential.  Phi(-|z|) of GELU is half of Abramowitz & Stegun 7.1.26 (erfc to 1.5e-7, from
 // the same e^(-z^2/2) as the density): a library erf costs four times the instructions, and 67 M of them took as long as the
 // product of 16384 x 1024 x 4096 itself.
-__device__ __forceinline__ float la_act(float z, int act, float* slope) {
-  float y = z, s = 1.f;
-  switch (act) {
-    case VG_ACT_LRELU: s = z > 0.f ? 1.f : VG_LRELU_SLOPE; y = z * s; break;
-    case VG_ACT_SIGMOID: y = __builtin_amdgcn_rcpf(1.f + __expf(-z)); s = y * (1.f - y); break;
-    case VG_ACT_GELU: {
-      const float e = __expf(-0.5f * z * z), t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * fabsf(z));
-      const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-      const float phi = z < 0.f ? q : 1.f - q;
-      y = z * phi;
-      s = phi + z * e * 0.39894228040143268f;
+template <int N> __device__ __forceinline__ void la_act(float* z, int act, float* s) {
+  switch (act) {                                     // one branch for all N: their exponentials overlap
+    case VG_ACT_LRELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) { s[i] = z[i] > 0.f ? 1.f : VG_LRELU_SLOPE; z[i] *= s[i]; }
       break;
-    }
-    case VG_ACT_SILU: { const float p = __builtin_amdgcn_rcpf(1.f + __expf(-z)); y = z * p; s = p * (1.f + z * (1.f - p)); break; }
+    case VG_ACT_SIGMOID:
+#pragma unroll
+      for (int i = 0; i < N; ++i) { z[i] = __builtin_amdgcn_rcpf(1.f + __expf(-z[i])); s[i] = z[i] * (1.f - z[i]); }
+      break;
+    case VG_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float x = z[i], e = __expf(-0.5f * x * x), t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * fabsf(x));
+        const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float phi = x < 0.f ? q : 1.f - q;
+        z[i] = x * phi;
+        s[i] = phi + x * e * 0.39894228040143268f;
+      }
+      break;
+    case VG_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float x = z[i], p = __builtin_amdgcn_rcpf(1.f + __expf(-x));
+        z[i] = x * p;
+        s[i] = p * (1.f + x * (1.f - p));
+      }
+      break;
     default: break;
   }
-  *slope = s;
-  return y;
 }
 
 struct GemmParams {
@@ -91,8 +103,7 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
       for (int e = 0; e < 8; ++e) v[e] += t[e];
     }
     if (p.act != VG_ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = la_act(v[e], p.act, &s[e]);
+      la_act<8>(v, p.act, s);
       if (p.slope) put8((S*)p.slope + o, s);
     }
     if (p.res) {
@@ -105,9 +116,9 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (j + e >= p.n) continue;
-      float x = v[e], s;
+      float x = v[e], s = 1.f;
       if (p.bias) x += p.bias_f32 ? ((const float*)p.bias)[j + e] : (float)((const T*)p.bias)[j + e];
-      x = la_act(x, p.act, &s);
+      la_act<1>(&x, p.act, &s);
       if (p.slope) ((S*)p.slope)[o + e] = (S)s;
       if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j + e];
       if (p.c_f32) ((float*)p.c)[o + e] = x; else ((T*)p.c)[o + e] = (T)x;
