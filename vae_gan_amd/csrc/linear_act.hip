@@ -92,16 +92,22 @@ template <typename O> __device__ __forceinline__ void get8(const O* p, float* v)
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = (float)o[e];
 }
-template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v) {
+// the bias of columns j..j+7 (zeros without one): a lane keeps its columns from row to row
+template <typename T> __device__ __forceinline__ void la_bias8(const GemmParams& p, int j, float* t) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = 0.f;
+  if (!p.bias) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (j + e < p.n) t[e] = p.bias_f32 ? ((const float*)p.bias)[j + e] : (float)((const T*)p.bias)[j + e];
+}
+template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v, const float* bias) {
   typedef typename SlopeT<T>::type S;
   const int64_t o = (int64_t)i * p.n + j;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
   if (p.vec && j + 8 <= p.n) {
     float t[8], s[8];
-    if (p.bias) {
-      if (p.bias_f32) get8((const float*)p.bias + j, t); else get8((const T*)p.bias + j, t);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += t[e];
-    }
     if (p.act != VG_ACT_NONE) {
       la_act<8>(v, p.act, s);
       if (p.slope) put8((S*)p.slope + o, s);
@@ -117,7 +123,6 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
     for (int e = 0; e < 8; ++e) {
       if (j + e >= p.n) continue;
       float x = v[e], s = 1.f;
-      if (p.bias) x += p.bias_f32 ? ((const float*)p.bias)[j + e] : (float)((const T*)p.bias)[j + e];
       la_act<1>(&x, p.act, &s);
       if (p.slope) ((S*)p.slope)[o + e] = (S)s;
       if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j + e];
@@ -298,7 +303,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
   // acc[u][v][r] of a lane: row 16 u + lane % 16, column 16 v + 4 (lane / 16) + r.  Through LDS (half of the wave's rows at a
   // time), so that a lane finishes eight neighbouring columns and a row of the wave's tile leaves as one run of memory.
   constexpr int LDW = 16 * NT + 4, HALF = MT / 2;
+  static_assert(64 % (2 * NT) == 0, "a lane keeps its columns");
   float* st = (float*)smem + wave * 16 * HALF * LDW;
+  const int c = (lane % (2 * NT)) * 8, j = j0 + wn * NT * 16 + c;
+  float bias[8];
+  if (!p.part) la_bias8<T>(p, j, bias);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -308,16 +317,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 1
-    for (int q = lane; q < 32 * NT * HALF; q += 64) {
-      const int r = q / (2 * NT), c = (q % (2 * NT)) * 8;
-      const int i = i0 + (wm * MT + h * HALF) * 16 + r, j = j0 + wn * NT * 16 + c;
+#pragma unroll 4
+    for (int t = 0; t < NT * HALF / 2; ++t) {
+      const int r = (t * 64 + lane) / (2 * NT);
+      const int i = i0 + (wm * MT + h * HALF) * 16 + r;
       float v[8];
       *(f32x4*)v = *(const f32x4*)(st + r * LDW + c);
       *(f32x4*)(v + 4) = *(const f32x4*)(st + r * LDW + c + 4);
       if (i < p.m && j < p.n) {
         if (p.part) put8(p.part + ((int64_t)split * p.m + i) * p.ldp + j, v);
-        else la_finish8<T>(p, i, j, v);
+        else la_finish8<T>(p, i, j, v, bias);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -339,7 +348,9 @@ template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(co
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
   }
-  la_finish8<T>(p, i, j, v);
+  float bias[8];
+  la_bias8<T>(p, j, bias);
+  la_finish8<T>(p, i, j, v, bias);
 }
 
 // [rows][cols] (row stride ld) into [rows][pitch], the padding zeroed; S -> T rounds (an f32 master weight for bf16 products)
@@ -356,26 +367,45 @@ __global__ __launch_bounds__(256) void la_pack_kernel(const S* __restrict__ src,
   }
 }
 
-// dz = dy slope (dz = dy without one) and partial column sums of the unrounded dz: part[row chunk][n]
-template <typename T>
+// dz = dy slope (dz = dy without one) and partial column sums of the unrounded dz: part[row chunk][n].
+// VEC 8: a block is 32 column groups of 8 (512 bytes of a row) by 8 rows, so 16-byte accesses and runs of memory; bound by
+// one read of dy and slope and one write of dz.
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, const typename SlopeT<T>::type* __restrict__ slope, T* __restrict__ dz,
                                                     float* __restrict__ part, int m, int n, int rows_per) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
+  __shared__ float fold[8][32 * VEC + 1];
+  const int cg = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int j = (blockIdx.x * 32 + cg) * VEC;
   const int r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < m ? r0 + rows_per : m;
-  float s = 0.f;
-  for (int r = r0; r < r1; ++r) {
-    const int64_t o = (int64_t)r * n + j;
-    float g = (float)dy[o];
-    if (slope) {
-      g *= (float)slope[o];
-      dz[o] = (T)g;
+  float s[VEC] = {};
+  if (j < n) {
+#pragma unroll 4
+    for (int r = r0 + ry; r < r1; r += 8) {
+      const int64_t o = (int64_t)r * n + j;
+      float g[VEC], t[VEC];
+      if constexpr (VEC == 8) get8(dy + o, g); else g[0] = (float)dy[o];
+      if (slope) {
+        if constexpr (VEC == 8) get8(slope + o, t); else t[0] = (float)slope[o];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] *= t[e];
+        if constexpr (VEC == 8) put8(dz + o, g); else dz[o] = (T)g[0];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] += g[e];
     }
-    s += g;
   }
-  if (part) part[(int64_t)blockIdx.y * n + j] = s;
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) fold[ry][cg * VEC + e] = s[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * VEC; c += 256) {
+    const int col = blockIdx.x * 32 * VEC + c;
+    float t = fold[0][c];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) t += fold[q][c];
+    if (col < n) part[(int64_t)blockIdx.y * n + col] = t;
+  }
 }
-
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 // An operand as the tiles read it: the caller's matrix where it has 16-byte rows, otherwise a zero-padded copy.
@@ -392,24 +422,27 @@ static bool la_direct(const LaOperand& o, int dtype) {
 }
 static size_t la_packed_bytes(const LaOperand& o, int dtype) { return la_up((size_t)o.rows * la_pitch(o.cols) * vg_elt_size(dtype)); }
 
-// which tiles, and how many ways the contraction is split
+// Which tiles, and how many ways the contraction is split (partial sums in f32, joined by a kernel): the cheapest by
+//   rounds of blocks over the chip * (128-byte steps of k * step + fixed)  +  traffic and launch of the join
+// with the measured times (us) of a step and of a block's ends: 256 x 256 (one block a CU) 1.7 and 7, 128 x 128 (two) 1.15 and 5,
+// f32 128 x 128 4.1 and 5.  E.g. dW of 16384 x 1024 x 4096: 128 x 128 in two parts 187 us, 256 x 256 in four 158.
 struct LaPlan { int big, splits, ktiles; };
 static LaPlan la_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   const int64_t kt = vg_ceil_div(k * vg_elt_size(dtype), 128);
-  LaPlan p;
-  const int64_t t256 = vg_ceil_div(m, 256) * vg_ceil_div(n, 256), t128 = vg_ceil_div(m, 128) * vg_ceil_div(n, 128);
-  p.big = dtype == VG_BF16 && t256 >= 200;
-  const int64_t tiles = p.big ? t256 : t128, slots = p.big ? 256 : 512;
-  int64_t s = 1;
-  if (tiles * 2 <= slots) {
-    s = slots / tiles;
-    if (s > kt / 4) s = kt / 4;                      // at least 4 tiles of k a split
-    if (s > 32) s = 32;
-    if (s < 1) s = 1;
+  LaPlan best = {0, 1, (int)kt};
+  double least = 1e30;
+  for (int big = 0; big <= (dtype == VG_BF16 ? 1 : 0); ++big) {
+    const int64_t tiles = big ? vg_ceil_div(m, 256) * vg_ceil_div(n, 256) : vg_ceil_div(m, 128) * vg_ceil_div(n, 128);
+    const int64_t slots = big ? 256 : 512;
+    const double step = dtype == VG_F32 ? 4.1 : big ? 1.7 : 1.15, fixed = big ? 7 : 5;
+    for (int64_t s = 1; s <= 32 && (s == 1 || kt / s >= 4); s += s < 4 ? 1 : s < 8 ? 2 : 4) {
+      const int64_t per = vg_ceil_div(kt, s), parts = vg_ceil_div(kt, per);
+      const double join = parts > 1 ? 4 + (double)parts * m * n * 8 / 4.5e6 : 0;
+      const double t = vg_ceil_div(tiles * parts, slots) * (per * step + fixed) + join;
+      if (t < least) { least = t; best = {big, (int)parts, (int)per}; }
+    }
   }
-  p.ktiles = (int)vg_ceil_div(kt, s);
-  p.splits = (int)vg_ceil_div(kt, p.ktiles);
-  return p;
+  return best;
 }
 static size_t la_part_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   const LaPlan pl = la_plan(m, n, k, dtype);
@@ -505,23 +538,28 @@ extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int 
   return la_gemm(p, {x, ldx, m, k, 0}, false, {w, k, n, k, w_dtype == VG_F32}, false, dtype, ws, (hipStream_t)stream);
 }
 
-static const int LA_DZ_PARTS = 256;
+// chunks of rows: enough blocks to fill the chip, at least 32 rows each so that the partial sums stay a small part of the traffic
+static int la_dz_parts(int64_t m, int64_t n) {
+  int64_t parts = vg_ceil_div(2048, vg_ceil_div(n, 256));
+  if (parts > vg_ceil_div(m, 32)) parts = vg_ceil_div(m, 32);
+  return (int)parts;
+}
 extern "C" size_t vg_linear_act_dz_ws_bytes(int64_t m, int64_t n) {
-  return (size_t)(m < LA_DZ_PARTS ? m : LA_DZ_PARTS) * (size_t)n * sizeof(float);
+  return m < 1 || n < 1 ? 0 : (size_t)la_dz_parts(m, n) * (size_t)n * sizeof(float);
 }
 extern "C" int vg_linear_act_dz(const void* dy, const void* slope, void* dz, void* db, int bias_dtype, void* ws, int64_t m, int64_t n,
                                 int dtype, void* stream) {
   if (int rc = la_check("linear_act_dz", m, n, 1, VG_ACT_NONE, dtype)) return rc;
   VG_REQUIRE(dy && (!slope || dz) && (slope || db) && (!db || ws), "linear_act_dz: null pointer");
   hipStream_t st = (hipStream_t)stream;
-  int parts = (int)(m < LA_DZ_PARTS ? m : LA_DZ_PARTS);
-  const int per = (int)vg_ceil_div(m, parts);
-  parts = (int)vg_ceil_div(m, per);
-  const dim3 grid((unsigned)vg_ceil_div(n, 256), (unsigned)parts);
+  const int per = (int)vg_ceil_div(m, la_dz_parts(m, n)), parts = (int)vg_ceil_div(m, per);
   float* part = db ? (float*)ws : nullptr;
-  if (dtype == VG_BF16)
-    hipLaunchKernelGGL(la_dz_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)dy, (const f16_t*)slope, (bf16_t*)dz, part, (int)m, (int)n, per);
-  else hipLaunchKernelGGL(la_dz_kernel<float>, grid, dim3(256), 0, st, (const float*)dy, (const float*)slope, (float*)dz, part, (int)m, (int)n, per);
+  const bool vec = n % 8 == 0 && ((uintptr_t)dy | (uintptr_t)slope | (uintptr_t)dz) % 16 == 0;
+  const dim3 grid((unsigned)vg_ceil_div(n, vec ? 256 : 32), (unsigned)parts);
+#define LA_DZ(T, V) hipLaunchKernelGGL((la_dz_kernel<T, V>), grid, dim3(256), 0, st, (const T*)dy, (const SlopeT<T>::type*)slope, (T*)dz, part, (int)m, (int)n, per)
+  if (dtype == VG_BF16) { if (vec) LA_DZ(bf16_t, 8); else LA_DZ(bf16_t, 1); }
+  else { if (vec) LA_DZ(float, 8); else LA_DZ(float, 1); }
+#undef LA_DZ
   VG_LAUNCH_CHECK();
   if (db) return vg_fold_cols(part, parts, n, db, n, nullptr, bias_dtype, st);
   return VG_OK;

@@ -46,51 +46,60 @@ template <typename T, int VEC, int GL, int NV>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
                                                      const float* __restrict__ b, T* __restrict__ y, int64_t ldy,
                                                      float* __restrict__ stats, int64_t rows, int c, int cs, float eps) {
-  __shared__ float red[8];
+  __shared__ float red[16];
   constexpr int RPB = 256 / GL;
   const int gl = threadIdx.x % GL;
-  const int64_t row = blockIdx.x * (int64_t)RPB + threadIdx.x / GL;
-  const bool live = row < rows;                       // dead groups still take part in the shuffles and barriers
-  float v[NV][VEC];
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * GL + gl) * VEC;
-    if (live && col < cs) ld_vec<T, VEC>(x + row * ldx + col, v[i]);
-    else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s += col + e < c ? v[i][e] : 0.f;
-  }
   const float inv = 1.f / (float)c;
-  const float mu = row_sum<GL>(s, red, 0) * inv;
-  float q = 0.f;
+  float wv[NV][VEC], bv[NV][VEC];                    // zero in the padding: y comes out as 0 there
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * GL + gl) * VEC;
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float d = v[i][e] - mu;
-      q += col + e < c ? d * d : 0.f;
+      const int col = (i * GL + gl) * VEC + e;
+      wv[i][e] = col < c ? w[col] : 0.f;
+      bv[i][e] = col < c ? b[col] : 0.f;
     }
-  }
-  const float var = row_sum<GL>(q, red, 1) * inv;
-  const float r = 1.f / sqrtf(var + eps);
-  if (!live) return;
-  if (stats && gl == 0) { stats[2 * row] = mu; stats[2 * row + 1] = r; }
+  int turn = 0;
+  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 2) {
+    const int64_t row = r0 + threadIdx.x / GL;
+    const bool live = row < rows;                     // dead groups still take part in the shuffles and barriers
+    float v[NV][VEC];
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * GL + gl) * VEC;
-    if (col >= cs) break;
-    float o[VEC];
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * GL + gl) * VEC;
+      if (live && col < cs) ld_vec<T, VEC>(x + row * ldx + col, v[i]);
+      else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const bool in = col + e < c;
-      o[e] = in ? (v[i][e] - mu) * r * w[in ? col + e : 0] + b[in ? col + e : 0] : 0.f;
+        for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (col + e >= c) v[i][e] = 0.f;
+        s += v[i][e];
+      }
     }
-    st_vec<T, VEC>(y + row * ldy + col, o);
+    const float mu = row_sum<GL>(s, red, turn) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[i][e] -= mu;
+        q += (i * GL + gl) * VEC + e < c ? v[i][e] * v[i][e] : 0.f;
+      }
+    const float r = 1.f / sqrtf(row_sum<GL>(q, red, turn + 1) * inv + eps);
+    if (!live) continue;
+    if (stats && gl == 0) { stats[2 * row] = mu; stats[2 * row + 1] = r; }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * GL + gl) * VEC;
+      if (col >= cs) break;
+      float o[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = col + e < c ? v[i][e] * r * wv[i][e] + bv[i][e] : 0.f;
+      st_vec<T, VEC>(y + row * ldy + col, o);
+    }
   }
 }
 
@@ -239,22 +248,24 @@ __global__ __launch_bounds__(256) void ln_bwd_long_params_kernel(const T* __rest
   part[(size_t)blockIdx.y * 2 * c + c + col] = d;
 }
 
-// out[col] = sum over parts of part[p][col], in the order of p within each of 8 interleaved groups, then the groups in order
+// out[col] = sum over parts of part[p][col]: 32 interleaved chains of parts a column, then the chains in order
 template <typename O>
-__global__ __launch_bounds__(256) void fold_cols_kernel(const float* __restrict__ part, int parts, int64_t cols, int64_t stride,
-                                                        O* __restrict__ out0, int64_t split, O* __restrict__ out1) {
-  __shared__ float s[8][32];
+__global__ __launch_bounds__(1024) void fold_cols_kernel(const float* __restrict__ part, int parts, int64_t cols, O* __restrict__ out0,
+                                                         int64_t split, O* __restrict__ out1) {
+  __shared__ float s[32][33];
   const int cx = threadIdx.x & 31, py = threadIdx.x >> 5;
   const int64_t col = blockIdx.x * (int64_t)32 + cx;
   float a = 0.f;
-  if (col < cols)
-    for (int p = py; p < parts; p += 8) a += part[p * stride + col];
+  if (col < cols) {
+#pragma unroll 8
+    for (int p = py; p < parts; p += 32) a += part[p * cols + col];
+  }
   s[py][cx] = a;
   __syncthreads();
   if (py == 0 && col < cols) {
     float t = s[0][cx];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) t += s[i][cx];
+    for (int i = 1; i < 32; ++i) t += s[i][cx];
     O* o = col < split ? out0 + col : out1 + (col - split);
     if (col < split ? out0 != nullptr : out1 != nullptr) *o = (O)t;
   }
@@ -263,8 +274,8 @@ __global__ __launch_bounds__(256) void fold_cols_kernel(const float* __restrict_
 int vg_fold_cols(const float* part, int parts, int64_t cols, void* out0, int64_t split, void* out1, int dtype, hipStream_t st) {
   const dim3 grid((unsigned)vg_ceil_div(cols, 32));
   if (dtype == VG_BF16)
-    hipLaunchKernelGGL(fold_cols_kernel<bf16_t>, grid, dim3(256), 0, st, part, parts, cols, cols, (bf16_t*)out0, split, (bf16_t*)out1);
-  else hipLaunchKernelGGL(fold_cols_kernel<float>, grid, dim3(256), 0, st, part, parts, cols, cols, (float*)out0, split, (float*)out1);
+    hipLaunchKernelGGL(fold_cols_kernel<bf16_t>, grid, dim3(1024), 0, st, part, parts, cols, (bf16_t*)out0, split, (bf16_t*)out1);
+  else hipLaunchKernelGGL(fold_cols_kernel<float>, grid, dim3(1024), 0, st, part, parts, cols, (float*)out0, split, (float*)out1);
   VG_LAUNCH_CHECK();
   return VG_OK;
 }
@@ -273,7 +284,12 @@ int vg_fold_cols(const float* part, int parts, int64_t cols, void* out0, int64_t
 // blocks of the backward pass: enough to fill the chip, few enough that the partial sums (8 c bytes a block) stay small
 static int64_t ln_bwd_blocks(int64_t rows, int rpb) {
   const int64_t need = vg_ceil_div(rows, rpb);
-  return need < 1024 ? need : 1024;
+  return need < 768 ? need : 768;
+}
+// forward: a block keeps the weights of its columns over several rows
+static int64_t ln_fwd_blocks(int64_t rows, int rpb) {
+  const int64_t need = vg_ceil_div(rows, rpb);
+  return need < 2048 ? need : 2048;
 }
 static const int LN_LONG_PARTS = 64;
 
@@ -293,7 +309,7 @@ struct LnArgs {
 template <typename T, int VEC, int GL, int NV> static void ln_launch(const LnArgs& a, bool bwd, hipStream_t st) {
   constexpr int RPB = 256 / GL;
   if (!bwd)
-    hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, GL, NV>), dim3((unsigned)vg_ceil_div(a.rows, RPB)), dim3(256), 0, st, (const T*)a.x,
+    hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, GL, NV>), dim3((unsigned)ln_fwd_blocks(a.rows, RPB)), dim3(256), 0, st, (const T*)a.x,
                        a.ldx, a.w, a.b, (T*)a.out, a.ldo, a.stats, a.rows, a.c, a.cs, a.eps);
   else
     hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, GL, NV>), dim3((unsigned)ln_bwd_blocks(a.rows, RPB)), dim3(256),
