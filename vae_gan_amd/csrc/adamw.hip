@@ -7,6 +7,7 @@
 // are rounded.  A scale that follows the largest value (not a power of two) lets a block of unchanging codes decay.
 // Bound by memory: 28 bytes a parameter at 32 bits, 16.06 at 8.
 #include "common.h"
+#include "rows.h"
 
 #define ADAMW_BLOCK 256
 
@@ -51,18 +52,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwParams a, float* 
   }
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
 __device__ __forceinline__ float finite_abs(float v) { const float a = fabsf(v); return a < __builtin_inff() ? a : 0.f; }
 
 // a wave's 256 values as e4m3 codes and their scale.  Values that are not finite get the NaN code and do not set the scale
 // (the other elements of the block keep theirs).  The scale stays at least 2^-126, so its reciprocal is finite.
 template <bool ROOT> __device__ __forceinline__ unsigned encode8(const f32x4& v, float& scale) {
   float most = fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])));
-  scale = fmaxf(wave_max(most) * (1.f / 448.f), 0x1p-126f);
+  scale = fmaxf(wave_max64(most) * (1.f / 448.f), 0x1p-126f);
   const float inv = 1.f / scale;
   float q[4];
 #pragma unroll

@@ -7,50 +7,47 @@
 // NaN or +inf in a row makes its logp, H and gradient NaN.  tokens[r] == ignore: logp 0 and no gradient through logp; any
 // other token outside [0, vocab) gives logp NaN and no gradient through logp (it is never used as an index).
 #include "common.h"
+#include "rows.h"
 
 #define LP_MAX_TOP 32
 #define LP_CAND 512        // candidates a block can hold for the selection of the best
 
 template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
 
+// A set's maximum m, s = sum 2^d and u = sum 2^d d with d = (x - m) log2 e: one fused multiply-add and one exponential an
+// element.  Masked elements have d = -inf: clamped where it multiplies, since 0 * -inf is NaN (2^-290 is 0 in f32).
+#define LP_LOG2E 1.4426950408889634f
+#define LP_LN2 0.6931471805599453f
 struct Soft { float m, s, u; };
 __device__ __forceinline__ float safe_max(float m) { return m == -__builtin_inff() ? 0.f : m; }
+// the same set about another maximum
+__device__ __forceinline__ Soft soft_about(const Soft& a, float m) {
+  const float d = fmaxf((a.m - safe_max(m)) * LP_LOG2E, -290.f), e = __builtin_amdgcn_exp2f(d);
+  return Soft{m, a.s * e, e * (a.u + d * a.s)};
+}
 // (m, s, u) of two disjoint sets
 __device__ __forceinline__ Soft soft_join(const Soft& a, const Soft& b) {
-  Soft r;
-  r.m = fmaxf(a.m, b.m);
-  const float base = safe_max(r.m);
-  const float da = fmaxf(a.m - base, -200.f), db = fmaxf(b.m - base, -200.f);      // e^-200 is 0 in f32; an empty set has s = u = 0
-  const float ea = __expf(da), eb = __expf(db);
-  r.s = a.s * ea + b.s * eb;
-  r.u = ea * (a.u + da * a.s) + eb * (b.u + db * b.s);
-  return r;
+  const float m = fmaxf(a.m, b.m);
+  const Soft p = soft_about(a, m), q = soft_about(b, m);
+  return Soft{m, p.s + q.s, p.u + q.u};
 }
-__device__ __forceinline__ void soft_add(Soft& a, float x) {
-  const float d = x - safe_max(a.m), e = __expf(d);
+__device__ __forceinline__ void soft_add(Soft& a, float x, float base) {
+  const float d = (x - base) * LP_LOG2E, e = __builtin_amdgcn_exp2f(d);
   a.s += e;
-  a.u += e * fmaxf(d, -200.f);                       // masked: 0 * -200, not 0 * -inf
+  a.u += e * fmaxf(d, -290.f);
 }
 template <int N> __device__ __forceinline__ void soft_add_n(Soft& a, const float* x) {
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-  if (mx > a.m) {
-    const float d = fmaxf(a.m - mx, -200.f), e = __expf(d);
-    a.u = e * (a.u + d * a.s);
-    a.s *= e;
-    a.m = mx;
-  }
+  if (mx > a.m) a = soft_about(a, mx);
+  const float base = safe_max(a.m);
 #pragma unroll
-  for (int i = 0; i < N; ++i) soft_add(a, x[i]);
+  for (int i = 0; i < N; ++i) soft_add(a, x[i], base);
 }
-__device__ __forceinline__ Soft soft_wave(Soft a) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    Soft b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.u, o, 64)};
-    a = soft_join(a, b);
-  }
-  return a;
+__device__ __forceinline__ Soft soft_wave(const Soft& a) {
+  const Soft b = soft_about(a, wave_max64(a.m));
+  return Soft{b.m, wave_sum64(b.s), wave_sum64(b.u)};
 }
 
 // order of the alternatives: by value, then by place (lower first); NaN ranks as -inf, -0 as +0.  A larger key is better.
@@ -74,6 +71,25 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k)
   return k;
 }
 
+// the `top` largest of n different keys, to put(k, key), by one wave
+template <typename F> __device__ __forceinline__ void best_of(const unsigned long long* keys, int n, int top, int lane, F put) {
+  if (n <= 64) {                                     // each lane counts the keys above its own
+    const unsigned long long mine = lane < n ? keys[lane] : 0;
+    int above = 0;
+    for (int q = 0; q < n; ++q) above += keys[q] > mine;
+    if (lane < n && mine && above < top) put(above, mine);
+    return;
+  }
+  unsigned long long last = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    unsigned long long b = 0;
+    for (int q = lane; q < n; q += 64)
+      if (keys[q] < last && keys[q] > b) b = keys[q];
+    last = wave_max_key(b);
+    if (lane == 0) put(k, last);
+  }
+}
+
 struct LpParams {
   const void* x;
   int64_t ldx;
@@ -92,7 +108,7 @@ __device__ __forceinline__ void finish_row(const LpParams& p, int64_t row, const
   const bool empty = a.m == -__builtin_inff() && a.s == 0.f;
   const float ls = logf(a.s);
   const int64_t t = p.tokens[row];
-  p.entropy[row] = empty ? 0.f : ls - a.u / a.s;
+  p.entropy[row] = empty ? 0.f : ls - a.u / a.s * LP_LN2;
   p.logp[row] = t == p.ignore ? 0.f : (t < 0 || t >= p.vocab) ? __builtin_nanf("") : empty ? -__builtin_inff() : (xt - a.m) - ls;
   if (p.lse) { p.lse[2 * row] = empty ? 0.f : a.m; p.lse[2 * row + 1] = empty ? __builtin_inff() : ls; }     // e^(x - m - inf) = 0: no gradient
 }
@@ -131,13 +147,12 @@ __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
   float mx = v[0];
 #pragma unroll
   for (int i = 1; i < NV * VEC; ++i) mx = fmaxf(mx, v[i]);
+  Soft a = {wave_max64(mx), 0.f, 0.f};
+  const float base = safe_max(a.m);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  Soft a = {mx, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < NV * VEC; ++i) soft_add(a, v[i]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { a.s += __shfl_xor(a.s, o, 64); a.u += __shfl_xor(a.u, o, 64); }
+  for (int i = 0; i < NV * VEC; ++i) soft_add(a, v[i], base);
+  a.s = wave_sum64(a.s);
+  a.u = wave_sum64(a.u);
   if (lane == 0) finish_row(p, row, a, token_logit<T>(p, row));
   unsigned long long last = ~0ull;
   for (int k = 0; k < p.top; ++k) {
@@ -215,19 +230,19 @@ __global__ __launch_bounds__(256) void lp_block_kernel(const LpParams p) {
   }
   if (!p.top) return;
   // The k-th largest of the threads' maxima bounds the k-th largest element from below: k different elements reach it.
-  // One wave finds it (thread maxima as keys, the thread's number as the place), then everything at or above it is gathered.
+  // One wave finds it bit by bit, then everything at or above it is gathered.
   if (wave == 0) {
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-      unsigned long long b = 0;
+    unsigned o[4], t = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned long long key = rank_key(tmax[q * 64 + lane], (unsigned)(q * 64 + lane));
-        if (key < last && key > b) b = key;
-      }
-      last = wave_max_key(b);
+    for (int q = 0; q < 4; ++q) o[q] = (unsigned)(rank_key(tmax[q * 64 + lane], 0) >> 32);
+    for (int bit = 31; bit >= 0; --bit) {            // the largest t that at least `top` of the 256 reach
+      const unsigned u = t | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) n += __popcll(__ballot(o[q] >= u));
+      if (n >= p.top) t = u;
     }
-    if (lane == 0) bound = key_value(last);
+    if (lane == 0) bound = key_value((unsigned long long)t << 32);
   }
   __syncthreads();
   const float low = bound;
@@ -247,16 +262,7 @@ __global__ __launch_bounds__(256) void lp_block_kernel(const LpParams p) {
   __syncthreads();
   const int n = count;
   if (n >= p.top && n <= LP_CAND) {
-    if (wave == 0) {
-      unsigned long long last = ~0ull;
-      for (int k = 0; k < p.top; ++k) {
-        unsigned long long b = 0;
-        for (int q = lane; q < n; q += 64)
-          if (cand[q] < last && cand[q] > b) b = cand[q];
-        last = wave_max_key(b);
-        if (lane == 0) win[k] = last;
-      }
-    }
+    if (wave == 0) best_of(cand, n, p.top, lane, [&](int k, unsigned long long key) { win[k] = key; });
   } else {
     // so many equal values (a constant row), or so few that can be ranked, that the list does not hold the answer: one scan a place
     unsigned long long last = ~0ull;
@@ -285,9 +291,17 @@ __global__ __launch_bounds__(256) void lp_block_kernel(const LpParams p) {
 }
 
 // the splits of one row
-template <typename T> __global__ __launch_bounds__(64) void lp_join_kernel(const LpParams p) {
-  const int lane = threadIdx.x;
+#define LP_JOIN 2048
+template <typename T> __global__ __launch_bounds__(256) void lp_join_kernel(const LpParams p) {
+  __shared__ unsigned long long keys[LP_JOIN];
+  const int lane = threadIdx.x & 63, n = p.splits * p.top;
   const int64_t row = blockIdx.x;
+  const unsigned long long* c = p.cand + row * n;
+  if (n <= LP_JOIN) {
+    for (int q = threadIdx.x; q < n; q += 256) keys[q] = c[q];
+    __syncthreads();
+  }
+  if (threadIdx.x >= 64) return;
   Soft a = {-__builtin_inff(), 0.f, 0.f};
   for (int s = lane; s < p.splits; s += 64) {
     const float* o = p.part + (row * p.splits + s) * 4;
@@ -295,15 +309,7 @@ template <typename T> __global__ __launch_bounds__(64) void lp_join_kernel(const
   }
   a = soft_wave(a);
   if (lane == 0) finish_row(p, row, a, token_logit<T>(p, row));
-  const unsigned long long* c = p.cand + row * p.splits * p.top;
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
-    unsigned long long b = 0;
-    for (int q = lane; q < p.splits * p.top; q += 64)
-      if (c[q] < last && c[q] > b) b = c[q];
-    last = wave_max_key(b);
-    if (lane == 0) put_top(p, row, k, last, a);
-  }
+  if (p.top) best_of(n <= LP_JOIN ? keys : c, n, p.top, lane, [&](int k, unsigned long long key) { put_top(p, row, k, key, a); });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
@@ -400,7 +406,7 @@ template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
     return;
   }
   hipLaunchKernelGGL(lp_block_kernel<T>, dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
-  if (p.splits > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)p.rows), dim3(64), 0, st, p);
+  if (p.splits > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)p.rows), dim3(256), 0, st, p);
 }
 
 extern "C" int vg_token_logprobs_fwd(const void* logits, int64_t ldx, const int64_t* tokens, int64_t ignore, int64_t rows, int vocab,

@@ -10,13 +10,35 @@
 #include "rows.h"
 
 
-template <typename T, int VEC> __device__ __forceinline__ void ld_vec(const T* p, float* o) {
+// VEC elements as loaded, so that the next row can be on its way while this one is worked on
+template <typename T, int VEC> struct Raw {
   typedef T vt __attribute__((ext_vector_type(VEC)));
-  if constexpr (VEC == 1) o[0] = (float)*p;
-  else {
-    const vt v = *(const vt*)p;
+  vt v;
+  __device__ __forceinline__ void load(const T* p) { v = *(const vt*)p; }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = (float)v[e];
+    for (int e = 0; e < VEC; ++e) v[e] = (T)0.f;
+  }
+  __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
+};
+template <typename T> struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void zero() { v = (T)0.f; }
+  __device__ __forceinline__ float get(int) const { return (float)v; }
+};
+// a lane's parameters, zero past c; 16-byte loads where the lane's columns allow them
+template <int VEC> __device__ __forceinline__ void ld_param(const float* w, int col, int c, float* o) {
+  if (VEC % 4 == 0 && col + VEC <= c && (uintptr_t)w % 16 == 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      const f32x4 q = *(const f32x4*)(w + col + e);
+#pragma unroll
+      for (int i = 0; i < (VEC < 4 ? VEC : 4); ++i) o[e + i] = q[i];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = col + e < c ? w[col + e] : 0.f;
   }
 }
 template <typename T, int VEC> __device__ __forceinline__ void st_vec(T* p, const float* o) {
@@ -32,8 +54,11 @@ template <typename T, int VEC> __device__ __forceinline__ void st_vec(T* p, cons
 
 // sum over the GL lanes that share a row; every lane gets it.  GL == 256: through LDS (red: one slot per wave and value)
 template <int GL> __device__ __forceinline__ float row_sum(float v, float* red, int slot) {
+  if constexpr (GL >= 64) v = wave_sum64(v);
+  else {
 #pragma unroll
-  for (int o = (GL < 64 ? GL : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int o = GL / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  }
   if constexpr (GL > 64) {
     if ((threadIdx.x & 63) == 0) red[slot * 4 + (threadIdx.x >> 6)] = v;
     __syncthreads();
@@ -52,33 +77,34 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, in
   const float inv = 1.f / (float)c;
   float wv[NV][VEC], bv[NV][VEC];                    // zero in the padding: y comes out as 0 there
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    ld_param<VEC>(w, (i * GL + gl) * VEC, c, wv[i]);
+    ld_param<VEC>(b, (i * GL + gl) * VEC, c, bv[i]);
+  }
+  Raw<T, VEC> in[NV];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = (i * GL + gl) * VEC + e;
-      wv[i][e] = col < c ? w[col] : 0.f;
-      bv[i][e] = col < c ? b[col] : 0.f;
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * GL + gl) * VEC;
+      if (row < rows && col < cs) in[i].load(x + row * ldx + col); else in[i].zero();
     }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
   int turn = 0;
-  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 2) {
+  fetch(blockIdx.x * (int64_t)RPB + threadIdx.x / GL);
+  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += step, turn ^= 2) {
     const int64_t row = r0 + threadIdx.x / GL;
     const bool live = row < rows;                     // dead groups still take part in the shuffles and barriers
     float v[NV][VEC];
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * GL + gl) * VEC;
-      if (live && col < cs) ld_vec<T, VEC>(x + row * ldx + col, v[i]);
-      else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
-      }
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        if (col + e >= c) v[i][e] = 0.f;
+        v[i][e] = (i * GL + gl) * VEC + e < c ? in[i].get(e) : 0.f;
         s += v[i][e];
       }
-    }
+    fetch(row + step);
     const float mu = row_sum<GL>(s, red, turn) * inv;
     float q = 0.f;
 #pragma unroll
@@ -134,31 +160,38 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ x, in
   const float inv = 1.f / (float)c;
   float aw[NV][VEC], ab[NV][VEC], wv[NV][VEC];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    ld_param<VEC>(w, (i * GL + gl) * VEC, c, wv[i]);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = (i * GL + gl) * VEC + e;
-      aw[i][e] = ab[i][e] = 0.f;
-      wv[i][e] = col < c ? w[col] : 0.f;
-    }
-  int turn = 0;
-  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 2) {
-    const int64_t row = r0 + threadIdx.x / GL;
+    for (int e = 0; e < VEC; ++e) aw[i][e] = ab[i][e] = 0.f;
+  }
+  Raw<T, VEC> nx[NV], ng[NV];
+  float nmu, nr;
+  auto fetch = [&](int64_t row) {
     const bool live = row < rows;
-    float xh[NV][VEC], g[NV][VEC];
-    const float mu = live ? stats[2 * row] : 0.f, r = live ? stats[2 * row + 1] : 0.f;
-    float sg = 0.f, sgx = 0.f;
+    nmu = live ? stats[2 * row] : 0.f;
+    nr = live ? stats[2 * row + 1] : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * GL + gl) * VEC;
-      if (live && col < cs) {
-        ld_vec<T, VEC>(x + row * ldx + col, xh[i]);
-        ld_vec<T, VEC>(dy + row * lddy + col, g[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) xh[i][e] = g[i][e] = 0.f;
-      }
+      if (live && col < cs) { nx[i].load(x + row * ldx + col); ng[i].load(dy + row * lddy + col); }
+      else { nx[i].zero(); ng[i].zero(); }
     }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int turn = 0;
+  fetch(blockIdx.x * (int64_t)RPB + threadIdx.x / GL);
+  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += step, turn ^= 2) {
+    const int64_t row = r0 + threadIdx.x / GL;
+    const bool live = row < rows;
+    float xh[NV][VEC], g[NV][VEC];
+    const float mu = nmu, r = nr;
+    float sg = 0.f, sgx = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) { xh[i][e] = nx[i].get(e); g[i][e] = ng[i].get(e); }
+    fetch(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * GL + gl) * VEC;
@@ -281,15 +314,16 @@ int vg_fold_cols(const float* part, int parts, int64_t cols, void* out0, int64_t
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
+static const int64_t LN_FWD_BLOCKS = 1024, LN_BWD_BLOCKS = 768;
 // blocks of the backward pass: enough to fill the chip, few enough that the partial sums (8 c bytes a block) stay small
 static int64_t ln_bwd_blocks(int64_t rows, int rpb) {
   const int64_t need = vg_ceil_div(rows, rpb);
-  return need < 768 ? need : 768;
+  return need < LN_BWD_BLOCKS ? need : LN_BWD_BLOCKS;
 }
 // forward: a block keeps the weights of its columns over several rows
 static int64_t ln_fwd_blocks(int64_t rows, int rpb) {
   const int64_t need = vg_ceil_div(rows, rpb);
-  return need < 2048 ? need : 2048;
+  return need < LN_FWD_BLOCKS ? need : LN_FWD_BLOCKS;
 }
 static const int LN_LONG_PARTS = 64;
 
@@ -373,7 +407,7 @@ extern "C" int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, con
 
 extern "C" size_t vg_layer_norm_bwd_ws_bytes(int64_t rows, int c) {
   // the most blocks any variant launches; long rows use LN_LONG_PARTS
-  int64_t parts = rows < 1024 ? rows : 1024;
+  int64_t parts = rows < LN_BWD_BLOCKS ? rows : LN_BWD_BLOCKS;
   if (parts < LN_LONG_PARTS) parts = LN_LONG_PARTS;
   return (size_t)parts * 2 * (size_t)c * sizeof(float);
 }
