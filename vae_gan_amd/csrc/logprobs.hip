@@ -1,5 +1,5 @@
 // Log probabilities of given tokens under rows of logits, with the entropy and the best alternatives, and their gradient.
-//   m = max x, s = sum e^(x-m), u = sum e^(x-m) (x-m):  lse = m + ln s,  logp = x_t - lse,  H = ln s - u / s
+//   m = max x, s = sum e^(x-m), u = sum e^(x-m) (x-m):  logp = (x_t - m) - ln s,  H = ln s - u / s
 //   dx_j = dlogp ([j = t] - p_j) - dH p_j (ln p_j + H),  p_j = e^(x_j - lse)
 // Bound by memory: the forward reads the logits once, keeping (m, s, u) as running values that are rescaled when a larger
 // maximum arrives; the backward reads them once more and writes the gradient.  Sums are f32; exponents are of x - m <= 0.
@@ -10,19 +10,29 @@
 #include "rows.h"
 
 #define LP_MAX_TOP 32
-#define LP_CAND 512        // candidates a block can hold for the selection of the best
+#define LP_CAND 512        // candidates a block (a wave: a quarter) can hold for the selection of the best
 
 template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
 
-// A set's maximum m, s = sum 2^d and u = sum 2^d d with d = (x - m) log2 e: one fused multiply-add and one exponential an
-// element.  Masked elements have d = -inf: clamped where it multiplies, since 0 * -inf is NaN (2^-290 is 0 in f32).
+// A set of logits: m (its maximum), s = sum 2^d and u = sum 2^d d with d = x log2 e - c, c = m log2 e as rounded to f32: one
+// fused multiply-add and one exponential an element.  The rounding of c is the same in every d, so it cancels in d - log2 s.
+// Where x log2 e may leave the f32 range (rows at the type's lowest value), d = (x - m) log2 e.  Masked elements have d = -inf:
+// clamped where it multiplies, since 0 * -inf is NaN (2^-290 is 0 in f32).
 #define LP_LOG2E 1.4426950408889634f
 #define LP_LN2 0.6931471805599453f
+#define LP_FAR 2e38f
 struct Soft { float m, s, u; };
-__device__ __forceinline__ float safe_max(float m) { return m == -__builtin_inff() ? 0.f : m; }
-// the same set about another maximum
+__device__ __forceinline__ float soft_base(float m) { return m == -__builtin_inff() ? 0.f : m; }
+__device__ __forceinline__ float soft_d(float x, float base) {
+  return fabsf(base) < LP_FAR ? fmaf(x, LP_LOG2E, -(base * LP_LOG2E)) : (x - base) * LP_LOG2E;
+}
+// the same set about a larger maximum: the difference of the two c as they were rounded (not contracted), or the rounding
+// of the old one would stay in its sums
 __device__ __forceinline__ Soft soft_about(const Soft& a, float m) {
-  const float d = fmaxf((a.m - safe_max(m)) * LP_LOG2E, -290.f), e = __builtin_amdgcn_exp2f(d);
+#pragma clang fp contract(off)
+  const float b = soft_base(m);
+  const bool near = fabsf(b) < LP_FAR && fabsf(a.m) < LP_FAR;
+  const float d = fmaxf(near ? a.m * LP_LOG2E - b * LP_LOG2E : (a.m - b) * LP_LOG2E, -290.f), e = __builtin_amdgcn_exp2f(d);
   return Soft{m, a.s * e, e * (a.u + d * a.s)};
 }
 // (m, s, u) of two disjoint sets
@@ -31,24 +41,34 @@ __device__ __forceinline__ Soft soft_join(const Soft& a, const Soft& b) {
   const Soft p = soft_about(a, m), q = soft_about(b, m);
   return Soft{m, p.s + q.s, p.u + q.u};
 }
-__device__ __forceinline__ void soft_add(Soft& a, float x, float base) {
-  const float d = (x - base) * LP_LOG2E, e = __builtin_amdgcn_exp2f(d);
-  a.s += e;
-  a.u += e * fmaxf(d, -290.f);
+template <int N> __device__ __forceinline__ void soft_add(Soft& a, const float* x) {
+  const float base = soft_base(a.m);
+  auto add = [&](float d) {
+    const float e = __builtin_amdgcn_exp2f(d);
+    a.s += e;
+    a.u += e * fmaxf(d, -290.f);
+  };
+  if (fabsf(base) < LP_FAR) {
+    const float c = base * LP_LOG2E;
+#pragma unroll
+    for (int i = 0; i < N; ++i) add(fmaf(x[i], LP_LOG2E, -c));
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) add((x[i] - base) * LP_LOG2E);
+  }
 }
 template <int N> __device__ __forceinline__ void soft_add_n(Soft& a, const float* x) {
-  float mx = x[0];
+  float m = x[0];
 #pragma unroll
-  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-  if (mx > a.m) a = soft_about(a, mx);
-  const float base = safe_max(a.m);
-#pragma unroll
-  for (int i = 0; i < N; ++i) soft_add(a, x[i], base);
+  for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+  if (m > a.m) a = soft_about(a, m);
+  soft_add<N>(a, x);
 }
 __device__ __forceinline__ Soft soft_wave(const Soft& a) {
   const Soft b = soft_about(a, wave_max64(a.m));
   return Soft{b.m, wave_sum64(b.s), wave_sum64(b.u)};
 }
+__device__ __forceinline__ bool soft_empty(const Soft& a) { return a.m == -__builtin_inff() && a.s == 0.f; }
 
 // order of the alternatives: by value, then by place (lower first); NaN ranks as -inf, -0 as +0.  A larger key is better.
 __device__ __forceinline__ unsigned long long rank_key(float x, unsigned at) {
@@ -104,17 +124,20 @@ struct LpParams {
   unsigned long long* cand;           // [rows][splits][top]: its best
 };
 
+// ln p of a logit: (d - log2 s) ln 2, with d as it was summed; of one that is far down, whose d overflows, x - m - ln s
+__device__ __forceinline__ float soft_lnp(float x, const Soft& a) {
+  return fabsf(x) < LP_FAR ? (soft_d(x, a.m) - log2f(a.s)) * LP_LN2 : (x - a.m) - log2f(a.s) * LP_LN2;
+}
 __device__ __forceinline__ void finish_row(const LpParams& p, int64_t row, const Soft& a, float xt) {
-  const bool empty = a.m == -__builtin_inff() && a.s == 0.f;
-  const float ls = logf(a.s);
+  const bool empty = soft_empty(a);
+  const float l2 = log2f(a.s);
   const int64_t t = p.tokens[row];
-  p.entropy[row] = empty ? 0.f : ls - a.u / a.s * LP_LN2;
-  p.logp[row] = t == p.ignore ? 0.f : (t < 0 || t >= p.vocab) ? __builtin_nanf("") : empty ? -__builtin_inff() : (xt - a.m) - ls;
-  if (p.lse) { p.lse[2 * row] = empty ? 0.f : a.m; p.lse[2 * row + 1] = empty ? __builtin_inff() : ls; }     // e^(x - m - inf) = 0: no gradient
+  p.entropy[row] = empty ? 0.f : (l2 - a.u / a.s) * LP_LN2;
+  p.logp[row] = t == p.ignore ? 0.f : (t < 0 || t >= p.vocab) ? __builtin_nanf("") : empty ? -__builtin_inff() : soft_lnp(xt, a);
+  if (p.lse) { p.lse[2 * row] = empty ? 0.f : a.m; p.lse[2 * row + 1] = empty ? __builtin_inff() : l2; }     // 2^(d - inf) = 0: no gradient
 }
 __device__ __forceinline__ void put_top(const LpParams& p, int64_t row, int i, unsigned long long key, const Soft& a) {
-  const bool empty = a.m == -__builtin_inff() && a.s == 0.f;
-  p.top_logp[row * p.top + i] = empty ? -__builtin_inff() : (key_value(key) - a.m) - logf(a.s);
+  p.top_logp[row * p.top + i] = soft_empty(a) ? -__builtin_inff() : soft_lnp(key_value(key), a);
   p.top_at[row * p.top + i] = key_place(key);
 }
 template <typename T> __device__ __forceinline__ float token_logit(const LpParams& p, int64_t row) {
@@ -148,9 +171,7 @@ __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
 #pragma unroll
   for (int i = 1; i < NV * VEC; ++i) mx = fmaxf(mx, v[i]);
   Soft a = {wave_max64(mx), 0.f, 0.f};
-  const float base = safe_max(a.m);
-#pragma unroll
-  for (int i = 0; i < NV * VEC; ++i) soft_add(a, v[i], base);
+  soft_add<NV * VEC>(a, v);
   a.s = wave_sum64(a.s);
   a.u = wave_sum64(a.u);
   if (lane == 0) finish_row(p, row, a, token_logit<T>(p, row));
@@ -171,123 +192,160 @@ __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
 }
 
 // ---- a block per row, or per split of a row -----------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void lp_block_kernel(const LpParams p) {
-  typedef T vt __attribute__((ext_vector_type(Elt<T>::PIECE)));
+// A unit (a row, or a split of one) belongs to a team: a wave, or the four waves of a block.
+template <int TEAM> __device__ __forceinline__ void team_sync() {
+  if constexpr (TEAM > 64) __syncthreads();
+  else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+template <int TEAM> struct LpLists {                 // of one team, in LDS
+  static constexpr int CAND = LP_CAND * TEAM / 256;
+  unsigned long long cand[CAND], best[4], win[LP_MAX_TOP];
+  float tmax[TEAM];
+  int count;
+  float bound;
+};
+template <typename T> struct LpUnit { const T* x; int64_t row; int split, j0, j1, a0, nvec; };
+
+// the best of one unit; mine: the maximum of this thread's elements, a: the unit's sums (its row's, where it is one)
+template <typename T, int TEAM>
+__device__ void lp_best(const LpParams& p, const LpUnit<T>& u, LpLists<TEAM>& l, float mine, const Soft& a) {
   constexpr int VEC = Elt<T>::PIECE;
-  __shared__ float sm[4][3], tmax[256];
-  __shared__ unsigned long long cand[LP_CAND], best[4], win[LP_MAX_TOP];
-  __shared__ int count;
-  __shared__ float bound;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x / p.splits;
-  const int split = (int)(blockIdx.x % p.splits);
-  const T* x = (const T*)p.x + row * p.ldx;
-  const int j0 = split * p.chunk, j1 = j0 + p.chunk < p.vocab ? j0 + p.chunk : p.vocab;
-  // head up to the first 16-byte boundary, whole accesses, tail
-  int h = (int)(((16 - (uintptr_t)(x + j0) % 16) % 16) / sizeof(T));
-  if (h > j1 - j0) h = j1 - j0;
-  const int a0 = j0 + h, nvec = (j1 - a0) / VEC, t0 = a0 + nvec * VEC;
-  Soft a = {-__builtin_inff(), 0.f, 0.f};
-  constexpr int U = 4;
-  int i = tid;
-  for (; i + (U - 1) * 256 < nvec; i += U * 256) {
-    float v[U * VEC];
+  typedef T vt __attribute__((ext_vector_type(VEC)));
+  const int tid = threadIdx.x % TEAM, lane = tid & 63, wave = tid >> 6, h = u.a0 - u.j0, t0 = u.a0 + u.nvec * VEC;
+  l.tmax[tid] = mine;
+  if (tid == 0) l.count = 0;
+  team_sync<TEAM>();
+  // The k-th largest of the threads' maxima bounds the k-th largest element from below: k different elements reach it.
+  // One wave finds it bit by bit, then everything at or above it is gathered.
+  if (wave == 0) {
+    unsigned o[TEAM / 64], t = 0;
+#pragma unroll
+    for (int q = 0; q < TEAM / 64; ++q) o[q] = (unsigned)(rank_key(l.tmax[q * 64 + lane], 0) >> 32);
+    for (int bit = 31; bit >= 0; --bit) {            // the largest t that at least `top` of the maxima reach
+      const unsigned v = t | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int q = 0; q < TEAM / 64; ++q) n += __popcll(__ballot(o[q] >= v));
+      if (n >= p.top) t = v;
+    }
+    if (lane == 0) l.bound = key_value((unsigned long long)t << 32);
+  }
+  team_sync<TEAM>();
+  const float low = l.bound;
+  auto gather = [&](float v, unsigned j) {
+    if ((v == v ? v : -__builtin_inff()) >= low) {
+      const int at = atomicAdd(&l.count, 1);
+      if (at < l.CAND) l.cand[at] = rank_key(v, j);
+    }
+  };
+  for (int q = tid; q < u.nvec; q += TEAM) {
+    const vt w = *(const vt*)(u.x + u.a0 + (int64_t)q * VEC);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) gather((float)w[e], (unsigned)(u.a0 + q * VEC + e));
+  }
+  if (tid < h) gather(ldf(u.x + u.j0 + tid), (unsigned)(u.j0 + tid));
+  if (tid < u.j1 - t0) gather(ldf(u.x + t0 + tid), (unsigned)(t0 + tid));
+  team_sync<TEAM>();
+  const int n = l.count;
+  if (n >= p.top && n <= l.CAND) {
+    if (wave == 0) best_of(l.cand, n, p.top, lane, [&](int k, unsigned long long key) { l.win[k] = key; });
+  } else {
+    // so many equal values (a constant row), or so few that can be ranked, that the list does not hold the answer: one scan a place
+    unsigned long long last = ~0ull;
+    for (int k = 0; k < p.top; ++k) {
+      unsigned long long b = 0;
+      for (int j = u.j0 + tid; j < u.j1; j += TEAM) {
+        const unsigned long long key = rank_key(ldf(u.x + j), (unsigned)j);
+        if (key < last && key > b) b = key;
+      }
+      b = wave_max_key(b);
+      if constexpr (TEAM > 64) {
+        if (lane == 0) l.best[wave] = b;
+        __syncthreads();
+        b = l.best[0];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) b = l.best[q] > b ? l.best[q] : b;
+        __syncthreads();
+      }
+      last = b;
+      if (tid == 0) l.win[k] = last;
+    }
+  }
+  team_sync<TEAM>();
+  if (tid < p.top) {
+    if (p.splits == 1) put_top(p, u.row, tid, l.win[tid], a);
+    else p.cand[(u.row * p.splits + u.split) * p.top + tid] = l.win[tid];
+  }
+}
+
+// The logits of a thread come in batches of U 16-byte accesses; the next batch is on its way while one is summed.
+template <typename T, int U, int TEAM>
+__global__ __launch_bounds__(256) void lp_row_kernel(const LpParams p) {
+  constexpr int VEC = Elt<T>::PIECE;
+  typedef T vt __attribute__((ext_vector_type(VEC)));
+  __shared__ float sm[4][3];
+  __shared__ LpLists<TEAM> lists[256 / TEAM];
+  const int tid = threadIdx.x % TEAM, lane = tid & 63, wave = tid >> 6;
+  const int64_t id = blockIdx.x * (int64_t)(256 / TEAM) + threadIdx.x / TEAM;
+  if (id >= p.rows * p.splits) return;               // a whole team: a block has one team or no barriers
+  LpUnit<T> u;
+  u.row = id / p.splits;
+  u.split = (int)(id % p.splits);
+  u.x = (const T*)p.x + u.row * p.ldx;
+  u.j0 = u.split * p.chunk;
+  u.j1 = u.j0 + p.chunk < p.vocab ? u.j0 + p.chunk : p.vocab;
+  const int h = (int)(((16 - (uintptr_t)(u.x + u.j0) % 16) % 16) / sizeof(T));      // elements before the first 16-byte boundary
+  u.a0 = u.j0 + (h < u.j1 - u.j0 ? h : u.j1 - u.j0);
+  u.nvec = (u.j1 - u.a0) / VEC;
+  vt next[U];
+  auto fetch = [&](int at) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const vt q = *(const vt*)(x + a0 + (int64_t)(i + k * 256) * VEC);
+      const int i = at + k * TEAM + tid;
+      if (i < u.nvec) next[k] = *(const vt*)(u.x + u.a0 + (int64_t)i * VEC);
+      else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[k * VEC + e] = (float)q[e];
+        for (int e = 0; e < VEC; ++e) next[k][e] = (T)(-__builtin_inff());
+      }
     }
-    soft_add_n<U * VEC>(a, v);
-  }
-  for (; i < nvec; i += 256) {
-    float v[VEC];
-    const vt q = *(const vt*)(x + a0 + (int64_t)i * VEC);
+  };
+  Soft a = {-__builtin_inff(), 0.f, 0.f};
+  fetch(0);
+  for (int at = U * TEAM;; at += U * TEAM) {
+    float v[U * VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = (float)q[e];
-    soft_add_n<VEC>(a, v);
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[k * VEC + e] = (float)next[k][e];
+    if (at < u.nvec) fetch(at);
+    soft_add_n<U * VEC>(a, v);
+    if (at >= u.nvec) break;
   }
-  if (tid < h) { const float v = ldf(x + j0 + tid); soft_add_n<1>(a, &v); }
-  if (tid < j1 - t0) { const float v = ldf(x + t0 + tid); soft_add_n<1>(a, &v); }
+  const int t0 = u.a0 + u.nvec * VEC;
+  if (tid < u.a0 - u.j0) { const float v = ldf(u.x + u.j0 + tid); soft_add_n<1>(a, &v); }
+  if (tid < u.j1 - t0) { const float v = ldf(u.x + t0 + tid); soft_add_n<1>(a, &v); }
   const float mine = a.m;
   a = soft_wave(a);
-  if (lane == 0) { sm[wave][0] = a.m; sm[wave][1] = a.s; sm[wave][2] = a.u; }
-  if (p.top) { tmax[tid] = mine; if (tid == 0) count = 0; }
-  __syncthreads();
-  {
+  if constexpr (TEAM > 64) {
+    if (lane == 0) { sm[wave][0] = a.m; sm[wave][1] = a.s; sm[wave][2] = a.u; }
+    __syncthreads();
     Soft q[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) q[k] = Soft{sm[k][0], sm[k][1], sm[k][2]};
     a = soft_join(soft_join(q[0], q[1]), soft_join(q[2], q[3]));
   }
   if (tid == 0) {
-    if (p.splits == 1) finish_row(p, row, a, token_logit<T>(p, row));
+    if (p.splits == 1) finish_row(p, u.row, a, token_logit<T>(p, u.row));
     else {
-      float* o = p.part + (row * p.splits + split) * 4;
+      float* o = p.part + (u.row * p.splits + u.split) * 4;
       o[0] = a.m; o[1] = a.s; o[2] = a.u;
     }
   }
-  if (!p.top) return;
-  // The k-th largest of the threads' maxima bounds the k-th largest element from below: k different elements reach it.
-  // One wave finds it bit by bit, then everything at or above it is gathered.
-  if (wave == 0) {
-    unsigned o[4], t = 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = (unsigned)(rank_key(tmax[q * 64 + lane], 0) >> 32);
-    for (int bit = 31; bit >= 0; --bit) {            // the largest t that at least `top` of the 256 reach
-      const unsigned u = t | 1u << bit;
-      int n = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) n += __popcll(__ballot(o[q] >= u));
-      if (n >= p.top) t = u;
-    }
-    if (lane == 0) bound = key_value((unsigned long long)t << 32);
-  }
-  __syncthreads();
-  const float low = bound;
-  auto gather = [&](float v, unsigned j) {
-    if ((v == v ? v : -__builtin_inff()) >= low) {
-      const int at = atomicAdd(&count, 1);
-      if (at < LP_CAND) cand[at] = rank_key(v, j);
-    }
-  };
-  for (int q = tid; q < nvec; q += 256) {
-    const vt w = *(const vt*)(x + a0 + (int64_t)q * VEC);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) gather((float)w[e], (unsigned)(a0 + q * VEC + e));
-  }
-  if (tid < h) gather(ldf(x + j0 + tid), (unsigned)(j0 + tid));
-  if (tid < j1 - t0) gather(ldf(x + t0 + tid), (unsigned)(t0 + tid));
-  __syncthreads();
-  const int n = count;
-  if (n >= p.top && n <= LP_CAND) {
-    if (wave == 0) best_of(cand, n, p.top, lane, [&](int k, unsigned long long key) { win[k] = key; });
-  } else {
-    // so many equal values (a constant row), or so few that can be ranked, that the list does not hold the answer: one scan a place
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-      unsigned long long b = 0;
-      for (int j = j0 + tid; j < j1; j += 256) {
-        const unsigned long long key = rank_key(ldf(x + j), (unsigned)j);
-        if (key < last && key > b) b = key;
-      }
-      b = wave_max_key(b);
-      if (lane == 0) best[wave] = b;
-      __syncthreads();
-      b = best[0];
-#pragma unroll
-      for (int q = 1; q < 4; ++q) b = best[q] > b ? best[q] : b;
-      last = b;
-      if (tid == 0) win[k] = last;
-      __syncthreads();
-    }
-  }
-  __syncthreads();
-  if (tid < p.top) {
-    if (p.splits == 1) put_top(p, row, tid, win[tid], a);
-    else p.cand[(row * p.splits + split) * p.top + tid] = win[tid];
-  }
+  if (p.top) lp_best<T, TEAM>(p, u, lists[threadIdx.x / TEAM], mine, a);
 }
 
 // the splits of one row
@@ -337,13 +395,12 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tp
   T* dx = (T*)p.dx + row * p.lddx;
   const int64_t t = p.tokens[row];
   const bool counts = t != p.ignore && t >= 0 && t < p.vocab;
-  const float m = p.lse[2 * row], ls = p.lse[2 * row + 1], h = p.entropy[row];
-  const bool empty = ls == __builtin_inff() && m == 0.f;
+  const float m = p.lse[2 * row], l2 = p.lse[2 * row + 1], h = p.entropy[row];
+  const bool empty = l2 == __builtin_inff() && m == 0.f;
   const float a = counts && p.dlogp && !empty ? p.dlogp[row] : 0.f, b = p.dent ? p.dent[row] : 0.f;
   auto grad = [&](float v, int j) {
-    const float lnp = (v - m) - ls;
-    const float e = __expf(lnp);
-    const float g = -e * (a + b * (fmaxf(lnp, -200.f) + h));
+    const float d = soft_d(v, m) - l2, e = __builtin_amdgcn_exp2f(d);
+    const float g = -e * (a + b * (fmaxf(d, -290.f) * LP_LN2 + h));
     return j == (int)t ? g + a : g;
   };
   int hd = (int)(((16 - (uintptr_t)(x + j0) % 16) % 16) / sizeof(T));
@@ -391,6 +448,7 @@ extern "C" size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top) {
   return s == 1 ? 0 : (size_t)rows * s * (4 * sizeof(float) + (size_t)top * 8);
 }
 
+static const int64_t LP_WAVE_UNITS = 2048;          // two waves a SIMD
 template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
   if (lp_regs(p.vocab)) {
     constexpr int V = Elt<T>::PIECE;
@@ -405,7 +463,13 @@ template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
 #undef LP_CASE
     return;
   }
-  hipLaunchKernelGGL(lp_block_kernel<T>, dim3((unsigned)(p.rows * p.splits)), dim3(256), 0, st, p);
+  // Many rows: a wave each, which leaves no barrier between loads and sums.  Few: a block each, with as many accesses in a
+  // batch as a unit has for each thread.
+  const int64_t units = p.rows * p.splits, per = vg_ceil_div(p.chunk < p.vocab ? p.chunk : p.vocab, 256 * Elt<T>::PIECE);
+  if (units >= LP_WAVE_UNITS) hipLaunchKernelGGL((lp_row_kernel<T, 4, 64>), dim3((unsigned)vg_ceil_div(units, 4)), dim3(256), 0, st, p);
+  else if (per == 1) hipLaunchKernelGGL((lp_row_kernel<T, 1, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
+  else if (per == 2) hipLaunchKernelGGL((lp_row_kernel<T, 2, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((lp_row_kernel<T, 4, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
   if (p.splits > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)p.rows), dim3(256), 0, st, p);
 }
 
