@@ -83,12 +83,9 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 }
 __device__ __forceinline__ unsigned key_place(unsigned long long k) { return 0xFFFFFFFFu - (unsigned)k; }
 __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned long long b = __shfl_xor(k, o, 64);
-    k = b > k ? b : k;
-  }
-  return k;
+  const unsigned hi = wave_umax64((unsigned)(k >> 32));       // the best value, then the best place among those that have it
+  const unsigned lo = wave_umax64((unsigned)(k >> 32) == hi ? (unsigned)k : 0u);
+  return ((unsigned long long)hi << 32) | lo;
 }
 
 // the `top` largest of n different keys, to put(k, key), by one wave
@@ -463,10 +460,11 @@ template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
 #undef LP_CASE
     return;
   }
-  // Many rows: a wave each, which leaves no barrier between loads and sums.  Few: a block each, with as many accesses in a
-  // batch as a unit has for each thread.
+  // Many rows: a wave each, which leaves no barrier between loads and sums, two accesses a batch (16384 x 8192 bf16: 52 us,
+  // 5.1 TB/s; a batch of four 72, since its registers halve the waves).  Few: a block each, with as many accesses in a batch
+  // as a unit has for each thread.
   const int64_t units = p.rows * p.splits, per = vg_ceil_div(p.chunk < p.vocab ? p.chunk : p.vocab, 256 * Elt<T>::PIECE);
-  if (units >= LP_WAVE_UNITS) hipLaunchKernelGGL((lp_row_kernel<T, 4, 64>), dim3((unsigned)vg_ceil_div(units, 4)), dim3(256), 0, st, p);
+  if (units >= LP_WAVE_UNITS) hipLaunchKernelGGL((lp_row_kernel<T, 2, 64>), dim3((unsigned)vg_ceil_div(units, 4)), dim3(256), 0, st, p);
   else if (per == 1) hipLaunchKernelGGL((lp_row_kernel<T, 1, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
   else if (per == 2) hipLaunchKernelGGL((lp_row_kernel<T, 2, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((lp_row_kernel<T, 4, 256>), dim3((unsigned)units), dim3(256), 0, st, p);

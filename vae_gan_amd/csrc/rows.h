@@ -30,3 +30,16 @@ __device__ __forceinline__ float wave_max64(float v) {
   v = fmaxf(v, wave_move<0x143, 0xc>(v, v));
   return wave_last(v);
 }
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned wave_umax_step(unsigned v) {
+  const unsigned o = (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xf, false);
+  return o > v ? o : v;
+}
+__device__ __forceinline__ unsigned wave_umax64(unsigned v) {
+  v = wave_umax_step<0x111, 0xf>(v);
+  v = wave_umax_step<0x112, 0xf>(v);
+  v = wave_umax_step<0x114, 0xf>(v);
+  v = wave_umax_step<0x118, 0xf>(v);
+  v = wave_umax_step<0x142, 0xa>(v);
+  v = wave_umax_step<0x143, 0xc>(v);
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
