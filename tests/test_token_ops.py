@@ -9,8 +9,8 @@ import torch
 @pytest.fixture(scope="module")
 def ops():
     from vae_gan_amd import lib as L
-    if not os.path.exists(L.LIB_PATH):
-        pytest.skip("libvg_hip.so not built")
+    if not os.path.exists(L.LIB_PATH) or not os.path.exists(os.path.join(os.path.dirname(L.LIB_PATH), "_vgtorch.so")):
+        pytest.skip("the libraries are not built")
     from vae_gan_amd import ops
     return ops
 

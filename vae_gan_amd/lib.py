@@ -164,6 +164,22 @@ def load() -> C.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The extension module with the autograd functions of the token-wise operators (csrc/torch_ops.cpp)."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _vgtorch
+        except ImportError as e:
+            raise RuntimeError(f"vae_gan_amd/_vgtorch.so cannot be loaded: build it with `make -C vae_gan_amd/csrc` ({e})") from e
+        _native = _vgtorch
+    return _native
+
+
 def last_error() -> str:
     return load().vg_last_error().decode("utf-8", "replace")
 

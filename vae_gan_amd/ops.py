@@ -14,7 +14,6 @@ import weakref
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib as L
 
@@ -1279,148 +1278,20 @@ def attention(q, k, v, x, gamma):
 
 
 # ----------------------------------------------------------------------------------------------
-# token-wise operators of a model of the code indices (csrc/norm.hip, linear_act.hip, logprobs.hip)
+# token-wise operators of a model of the code indices (csrc/norm.hip, linear_act.hip, logprobs.hip; autograd and argument
+# checks in csrc/torch_ops.cpp)
 # ----------------------------------------------------------------------------------------------
-def _on_device(what: str, x: torch.Tensor, *others):
-    """Checks that every tensor is on ``x``'s GPU; a context in which the launches go to that GPU's current stream."""
+def _on_device(what: str, x: torch.Tensor):
+    """A context in which launches go to the current stream of ``x``'s GPU."""
     _require_cuda(x, what)
-    for t in others:
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{what}: tensors on {x.device} and {t.device}")
     return torch.cuda.device(x.device) if x.device.index != torch.cuda.current_device() else contextlib.nullcontext()
-
-
-def _rows_of(t: torch.Tensor):
-    """``t`` as rows of its last dimension: a tensor [rows, c] whose rows are contiguous, and the row stride in elements.
-    A copy is made only where no single row stride describes ``t``."""
-    c = t.shape[-1]
-    r = t.reshape(-1, c)
-    if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < c):
-        r = r.contiguous()
-    return r, (r.stride(0) if r.shape[0] > 1 else c)
-
-
-class LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, c):
-        cs = x.shape[-1]
-        w, b = weight.contiguous(), bias.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        xr, ldx = _rows_of(x)
-        rows = xr.shape[0]
-        stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
-        with _on_device("layer_norm", x):
-            L.check(L.load().vg_layer_norm_fwd(xr.data_ptr(), ldx, w.data_ptr(), b.data_ptr(), y.data_ptr(), cs, L.ptr(stats), rows, c,
-                                               cs, eps, L.vg_dtype(x.dtype), L.stream()), "layer_norm_fwd")
-        ctx.save_for_backward(x, w, stats)
-        ctx.c = c
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, w, stats = ctx.saved_tensors
-        cs, c = x.shape[-1], ctx.c
-        xr, ldx = _rows_of(x)
-        gr, ldg = _rows_of(gy)
-        rows = xr.shape[0]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty(c, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[1] else None
-        db = torch.empty(c, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
-        if rows == 0:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
-        lib = L.load()
-        ws = None
-        if dw is not None or db is not None:
-            ws = torch.empty(lib.vg_layer_norm_bwd_ws_bytes(rows, c), dtype=torch.uint8, device=x.device)
-        with _on_device("layer_norm", x):
-            L.check(lib.vg_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, w.data_ptr(), stats.data_ptr(), dx.data_ptr(), cs,
-                                          L.ptr(dw), L.ptr(db), L.ptr(ws), rows, c, cs, L.vg_dtype(x.dtype), L.stream()), "layer_norm_bwd")
-        return dx, dw, db, None, None
 
 
 def layer_norm(x, weight, bias, eps: float = 1e-5, c: Optional[int] = None):
     """Layer norm over the first ``c`` of the last dimension's elements (default: all of them); the others, the channel
     padding of an NHWC tensor, come out as zeros and get no gradient.  ``x`` bf16 or f32 with any row stride; ``weight`` and
     ``bias`` f32 [c], as are their gradients."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"layer_norm: no columns in a tensor of shape {tuple(x.shape)}")
-    c = x.shape[-1] if c is None else int(c)
-    if not 1 <= c <= x.shape[-1]:
-        raise RuntimeError(f"layer_norm: c = {c} of {x.shape[-1]} columns")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t.dtype != torch.float32 or tuple(t.shape) != (c,):
-            raise RuntimeError(f"layer_norm: {name} must be float32 [{c}], got {t.dtype} {list(t.shape)}")
-    if eps < 0:
-        raise ValueError(f"layer_norm: eps = {eps}")
-    L.vg_dtype(x.dtype)
-    _on_device("layer_norm", x, weight, bias)
-    return LayerNormFn.apply(x, weight, bias, float(eps), c)
-
-
-def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-class LinearActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, act, residual):
-        lib = L.load()
-        dt, code, wcode = x.dtype, L.vg_dtype(x.dtype), L.vg_dtype(weight.dtype)
-        n, k = weight.shape
-        xr, ldx = _rows_of(x)
-        m = xr.shape[0]
-        y = torch.empty(*x.shape[:-1], n, dtype=dt, device=x.device)
-        w = weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        slope = None
-        if m:
-            rr, ldr = _rows_of(residual) if residual is not None else (None, 0)
-            if act != L.ACT_NONE and any(ctx.needs_input_grad[:3]):
-                slope = torch.empty(m, n, dtype=torch.float16 if dt == torch.bfloat16 else torch.float32, device=x.device)
-            ws = _workspace(lib.vg_linear_act_fwd_ws_bytes(xr.data_ptr(), ldx, w.data_ptr(), wcode, m, n, k, code), x.device)
-            with _on_device("linear_act", x):
-                L.check(lib.vg_linear_act_fwd(xr.data_ptr(), ldx, w.data_ptr(), wcode, L.ptr(b), 0 if b is None else L.vg_dtype(b.dtype),
-                                              L.ptr(rr), ldr, y.data_ptr(), L.ptr(slope), L.ptr(ws), m, n, k, act, code, L.stream()),
-                        "linear_act_fwd")
-        ctx.save_for_backward(x, w, slope)
-        ctx.bdt = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, w, slope = ctx.saved_tensors
-        lib = L.load()
-        dt, dev = x.dtype, x.device
-        code, wcode = L.vg_dtype(dt), L.vg_dtype(w.dtype)
-        n, k = w.shape
-        need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
-        xr, ldx = _rows_of(x)
-        m = xr.shape[0]
-        dx = torch.empty(x.shape, dtype=dt, device=dev) if need_x else None
-        dw = torch.empty(n, k, dtype=w.dtype, device=dev) if need_w else None
-        db = torch.empty(n, dtype=ctx.bdt, device=dev) if need_b else None
-        if m == 0:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, gy if need_r else None
-        g = gy.reshape(m, n).contiguous()
-        with _on_device("linear_act", x):
-            dz = g
-            if need_b or (slope is not None and (need_x or need_w)):
-                ws = _workspace(lib.vg_linear_act_dz_ws_bytes(m, n) if need_b else 0, dev)
-                if slope is not None:
-                    dz = torch.empty(m, n, dtype=dt, device=dev)
-                L.check(lib.vg_linear_act_dz(g.data_ptr(), L.ptr(slope), dz.data_ptr(), L.ptr(db), 0 if db is None else L.vg_dtype(ctx.bdt),
-                                             L.ptr(ws), m, n, code, L.stream()), "linear_act_dz")
-            if need_x:
-                ws = _workspace(lib.vg_linear_act_dgrad_ws_bytes(dz.data_ptr(), w.data_ptr(), wcode, m, n, k, code), dev)
-                L.check(lib.vg_linear_act_dgrad(dz.data_ptr(), w.data_ptr(), wcode, dx.data_ptr(), L.ptr(ws), m, n, k, code, L.stream()),
-                        "linear_act_dgrad")
-            if need_w:
-                ws = _workspace(lib.vg_linear_act_wgrad_ws_bytes(dz.data_ptr(), xr.data_ptr(), ldx, m, n, k, code), dev)
-                L.check(lib.vg_linear_act_wgrad(dz.data_ptr(), xr.data_ptr(), ldx, dw.data_ptr(), wcode, L.ptr(ws), m, n, k, code,
-                                                L.stream()), "linear_act_wgrad")
-        return dx, dw, db, None, gy if need_r else None
+    return L.native().layer_norm(x, weight, bias, eps, c)
 
 
 def linear_act(x, weight, bias=None, act: int = L.ACT_NONE, residual=None):
@@ -1429,72 +1300,7 @@ def linear_act(x, weight, bias=None, act: int = L.ACT_NONE, residual=None):
     weight for bf16 ``x`` (rounded to bf16 for the products; its gradient is f32).  ``bias`` [out] in ``x``'s dtype or f32;
     ``residual`` in ``x``'s dtype and the result's shape.  ``act``: ``L.ACT_NONE``, ``ACT_LRELU`` (0.2), ``ACT_SIGMOID``,
     ``ACT_GELU`` (z Phi(z)) or ``ACT_SILU``."""
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
-        raise RuntimeError(f"linear_act: mat1 and mat2 shapes cannot be multiplied ({list(x.shape)} and {list(weight.shape)} transposed)")
-    L.vg_dtype(x.dtype)
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"linear_act: {name} is {t.dtype}, x is {x.dtype} (the same or float32 is supported)")
-    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
-        raise RuntimeError(f"linear_act: bias of shape {list(bias.shape)} for {weight.shape[0]} outputs")
-    if residual is not None:
-        want = (*x.shape[:-1], weight.shape[0])
-        if residual.dtype != x.dtype or tuple(residual.shape) != want:
-            raise RuntimeError(f"linear_act: residual is {residual.dtype} {list(residual.shape)}, the result {x.dtype} {list(want)}")
-    if act not in (L.ACT_NONE, L.ACT_LRELU, L.ACT_SIGMOID, L.ACT_GELU, L.ACT_SILU):
-        raise ValueError(f"linear_act: activation {act}")
-    _on_device("linear_act", x, weight, bias, residual)
-    return LinearActFn.apply(x, weight, bias, int(act), residual)
-
-
-class TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top, ignore_index):
-        ctx.set_materialize_grads(False)
-        lib = L.load()
-        vocab, lead = logits.shape[-1], logits.shape[:-1]
-        xr, ldx = _rows_of(logits)
-        rows = xr.shape[0]
-        t = tokens.contiguous()
-        dev = logits.device
-        logp = torch.empty(lead, dtype=torch.float32, device=dev)
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        lse = torch.empty(rows, 2, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
-        top_logp = torch.empty(*lead, top, dtype=torch.float32, device=dev)
-        top_at = torch.empty(*lead, top, dtype=torch.int64, device=dev)
-        if rows:
-            nbytes = lib.vg_token_logprobs_ws_bytes(rows, vocab, top)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            with _on_device("token_logprobs", logits):
-                L.check(lib.vg_token_logprobs_fwd(xr.data_ptr(), ldx, t.data_ptr(), ignore_index, rows, vocab, top, logp.data_ptr(),
-                                                  entropy.data_ptr(), L.ptr(lse), top_logp.data_ptr(), top_at.data_ptr(), L.ptr(ws),
-                                                  L.vg_dtype(logits.dtype), L.stream()), "token_logprobs_fwd")
-        ctx.save_for_backward(logits, t, lse, entropy)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(top_logp, top_at)
-        return logp, entropy, top_logp, top_at
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logp, g_entropy, _top_logp, _top_at):
-        logits, t, lse, entropy = ctx.saved_tensors
-        vocab = logits.shape[-1]
-        xr, ldx = _rows_of(logits)
-        rows = xr.shape[0]
-        # rows laid out like the logits' own: the two are then aligned alike
-        ld = ldx if rows > 1 and ldx <= vocab + 256 else vocab
-        dx = torch.empty(rows, ld, dtype=logits.dtype, device=logits.device)[:, :vocab]
-        if rows and (g_logp is not None or g_entropy is not None):
-            ga = None if g_logp is None else g_logp.float().contiguous()
-            gb = None if g_entropy is None else g_entropy.float().contiguous()
-            with _on_device("token_logprobs", logits):
-                L.check(L.load().vg_token_logprobs_bwd(xr.data_ptr(), ldx, t.data_ptr(), ctx.ignore_index, lse.data_ptr(),
-                                                       entropy.data_ptr(), L.ptr(ga), L.ptr(gb), dx.data_ptr(), ld, rows, vocab,
-                                                       L.vg_dtype(logits.dtype), L.stream()), "token_logprobs_bwd")
-        return dx.reshape(logits.shape) if dx.is_contiguous() else dx.unflatten(0, logits.shape[:-1]), None, None, None
-
-
-TOP_MAX = 32
+    return L.native().linear_act(x, weight, bias, act, residual)
 
 
 def token_logprobs(logits, tokens, top: int = 0, ignore_index: int = -100):
@@ -1506,13 +1312,5 @@ def token_logprobs(logits, tokens, top: int = 0, ignore_index: int = -100):
     Logits of -inf are masked: no probability, no gradient.  A row of nothing else gives logp -inf, entropy 0 and gradient 0.
     NaN or +inf in a row gives NaN for it.  Positions whose token is ``ignore_index`` give logp 0 and take no gradient through
     it; any other token outside the vocabulary gives NaN (finding it here would need the host to wait for the GPU)."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise RuntimeError(f"token_logprobs: no logits in a tensor of shape {tuple(logits.shape)}")
-    if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1]:
-        raise RuntimeError(f"token_logprobs: tokens must be int64 {list(logits.shape[:-1])}, got {tokens.dtype} {list(tokens.shape)}")
-    if not 0 <= top <= min(TOP_MAX, logits.shape[-1]):
-        raise ValueError(f"token_logprobs: top = {top} of {logits.shape[-1]} logits (at most {TOP_MAX})")
-    L.vg_dtype(logits.dtype)
-    _on_device("token_logprobs", logits, tokens)
-    logp, entropy, top_logp, top_at = TokenLogprobsFn.apply(logits, tokens, int(top), int(ignore_index))
-    return (logp, entropy, top_logp, top_at) if top else (logp, entropy, None, None)
+    out = L.native().token_logprobs(logits, tokens, top, ignore_index)
+    return tuple(out) if top else (out[0], out[1], None, None)
