@@ -243,60 +243,65 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
   const int klimit = min(p.k, kt1 * KT);
   const unsigned lds0 = la_lds_addr(smem);
   int kload = kt0 * KT, slot = 0;
-  auto issue = [&]() {
-    const la_srd_t sa = la_srd(ga), sb = la_srd(gb);
-    const unsigned base = lds0 + slot * STAGE;
-#pragma unroll
-    for (int i = 0; i < TileA::LOADS; ++i) ta.load(i, sa, base, wave, kload, klimit);
-#pragma unroll
-    for (int i = 0; i < TileB::LOADS; ++i) tb.load(i, sb, base + TileA::BYTES, wave, kload, klimit);
+  la_srd_t srd_a, srd_b;
+  unsigned base;
+  auto begin = [&]() { srd_a = la_srd(ga); srd_b = la_srd(gb); base = lds0 + slot * STAGE; };
+  auto load = [&](int i) {
+    if (i < TileA::LOADS) ta.load(i, srd_a, base, wave, kload, klimit);
+    else tb.load(i - TileA::LOADS, srd_b, base + TileA::BYTES, wave, kload, klimit);
+  };
+  auto end = [&]() {
     if (kload + KT < klimit) { ga += TileA::step(p.lda); gb += TileB::step(p.ldb); }      // past the end only zeros are asked for
     kload += KT;
     slot = slot + 1 == S ? 0 : slot + 1;
   };
   f32x4 acc[MT][NT] = {};
   // Two sets of fragments: while the products of one half of a tile run, the other half (or the next tile's first half) is
-  // read from LDS.  Without that the eight waves read together and multiply together, and each unit idles half the time.
+  // read from LDS and the tile after the next is asked for, a few of each between the rows of products.  All reads first and
+  // all products after leaves each unit idle half of the time (8192 x 4096 x 4096: 248 us).
   u32x4 fa[2][MT], fb[2][NT];
-  auto read = [&](int set, const unsigned char* s, int ks) {
-#pragma unroll
-    for (int u = 0; u < MT; ++u) fa[set][u] = TileA::frag(s, wm * MT + u, ks, lane);
-#pragma unroll
-    for (int u = 0; u < NT; ++u) fb[set][u] = TileB::frag(s + TileA::BYTES, wn * NT + u, ks, lane);
+  auto read = [&](int set, const unsigned char* s, int ks, int i) {      // the columns' fragments first: every row needs them
+    if (i < NT) fb[set][i] = TileB::frag(s + TileA::BYTES, wn * NT + i, ks, lane);
+    else fa[set][i - NT] = TileA::frag(s, wm * MT + i - NT, ks, lane);
   };
-  auto multiply = [&](int set) {
+  constexpr int FRAGS = MT + NT, PER = (FRAGS + MT - 2) / (MT - 1), DMA = (LOADS + MT - 1) / MT;
+  auto multiply = [&](int set, const unsigned char* s, int ks, bool ask) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u)
+    for (int u = 0; u < MT; ++u) {
+      if (ask) {
+#pragma unroll
+        for (int i = u * DMA; i < (u + 1) * DMA && i < LOADS; ++i) load(i);
+      }
+#pragma unroll
+      for (int i = u * PER; i < (u + 1) * PER && i < FRAGS; ++i) read(set ^ 1, s, ks, i);
 #pragma unroll
       for (int v = 0; v < NT; ++v) acc[u][v] = la_mma<T>(fb[set][v], fa[set][u], acc[u][v]);
-  };
-  constexpr int READS = MT * TileA::FRAG_READS + NT * TileB::FRAG_READS, PRODUCTS = MT * NT * (sizeof(T) == 2 ? 1 : 4);
-  auto interleave = [&]() {                          // one LDS read every few products
-#pragma unroll
-    for (int i = 0; i < READS; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 #pragma unroll
-  for (int s = 0; s < S; ++s) issue();
+  for (int s = 0; s < S; ++s) {
+    begin();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(i);
+    end();
+  }
   la_wait_barrier<(S - 1) * LOADS>();
-  read(0, smem, 0);
+#pragma unroll
+  for (int i = 0; i < FRAGS; ++i) read(0, smem, 0, i);
   int cur = 0;
   auto next = [&]() {
     la_wait_barrier<(S - 2) * LOADS>();              // the next tile is in LDS, and everyone has read this one
-    issue();                                         // tile kt + S takes its place
     cur = cur + 1 == S ? 0 : cur + 1;
+    begin();                                         // tile kt + S takes its place
   };
   for (int kt = kt0; kt < kt1; kt += KB == 128 ? 1 : 2) {      // past the last tile: zeros
     if constexpr (KB == 64) next();
-    read(1, smem + cur * STAGE, KB == 64 ? 0 : 1);
-    multiply(0);
-    interleave();
+    multiply(0, smem + cur * STAGE, KB == 64 ? 0 : 1, KB == 64);
+    if constexpr (KB == 64) end();
     next();
-    read(0, smem + cur * STAGE, 0);
-    multiply(1);
-    interleave();
+    multiply(1, smem + cur * STAGE, 0, true);
+    end();
   }
   la_wait_barrier<0>();                              // the zeros asked for past the end have landed: LDS is free
 
