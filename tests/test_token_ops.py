@@ -139,8 +139,8 @@ def test_c_entry_points_return_an_error_instead_of_launching(ops):
     refused(la(act=7), "activation")
     refused(la(wdt=1), "weight dtype")
     refused(la(r=one, ldr=3), "row stride")
-    refused(la(k=7), "workspace")                      # rows that are not whole 16-byte pieces are copied first
-    refused(la(ws=one, k=7), "256")
+    refused(la(k=7, m=100), "workspace")               # rows that are not whole 16-byte pieces are copied first
+    refused(la(ws=one, k=7, m=100), "256")
     refused(lib.vg_linear_act_dz(one, None, one, None, 0, None, 1, 4, 0, None), "null")
     refused(lib.vg_linear_act_dz(one, one, one, one, 0, None, 1, 4, 0, None), "null")
     refused(lib.vg_linear_act_dgrad(one, None, 0, one, None, 1, 4, 8, 0, None), "null")

@@ -101,13 +101,23 @@ template <typename T> __device__ __forceinline__ void la_bias8(const GemmParams&
   for (int e = 0; e < 8; ++e)
     if (j + e < p.n) t[e] = p.bias_f32 ? ((const float*)p.bias)[j + e] : (float)((const T*)p.bias)[j + e];
 }
+template <typename T> __device__ __forceinline__ void la_finish1(const GemmParams& p, int i, int j, float x, float bias) {
+  typedef typename SlopeT<T>::type S;
+  const int64_t o = (int64_t)i * p.n + j;
+  float s = 1.f;
+  x += bias;
+  la_act<1>(&x, p.act, &s);
+  if (p.slope) ((S*)p.slope)[o] = (S)s;
+  if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j];
+  if (p.c_f32) ((float*)p.c)[o] = x; else ((T*)p.c)[o] = (T)x;
+}
 template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v, const float* bias) {
   typedef typename SlopeT<T>::type S;
   const int64_t o = (int64_t)i * p.n + j;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] += bias[e];
   if (p.vec && j + 8 <= p.n) {
     float t[8], s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += bias[e];
     if (p.act != VG_ACT_NONE) {
       la_act<8>(v, p.act, s);
       if (p.slope) put8((S*)p.slope + o, s);
@@ -120,14 +130,8 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
     if (p.c_f32) put8((float*)p.c + o, v); else put8((T*)p.c + o, v);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (j + e >= p.n) continue;
-      float x = v[e], s = 1.f;
-      la_act<1>(&x, p.act, &s);
-      if (p.slope) ((S*)p.slope)[o + e] = (S)s;
-      if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j + e];
-      if (p.c_f32) ((float*)p.c)[o + e] = x; else ((T*)p.c)[o + e] = (T)x;
-    }
+    for (int e = 0; e < 8; ++e)
+      if (j + e < p.n) la_finish1<T>(p, i, j + e, v[e], bias[e]);
   }
 }
 
@@ -340,6 +344,71 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
   }
 }
 
+// ---- few rows (m <= 64): one read of the weights -------------------------------------------------------------------------
+// A block takes 16 columns of C; its eight waves take k by turns of 4 x 64 bytes and join their sums in LDS, so the weights
+// stream from memory with 4 KB of each wave in flight and there is no second launch.  TW: f32 master weights are rounded here.
+// ALIGNED: rows of x and W begin at 16-byte boundaries and k is a whole number of pieces; otherwise elements are loaded one
+// by one.
+template <typename T, typename TW, bool ALIGNED> __device__ __forceinline__ u32x4 la_piece(const TW* row, int64_t k, int64_t kmax) {
+  constexpr int P = 16 / sizeof(T);
+  typedef T vt __attribute__((ext_vector_type(P)));
+  vt v;
+  if constexpr (ALIGNED) {
+    if (k >= kmax) return u32x4{0u, 0u, 0u, 0u};
+    if constexpr (sizeof(TW) == sizeof(T)) return *(const u32x4*)(row + k);
+    else {
+      const f32x4 a = *(const f32x4*)(row + k), b = *(const f32x4*)(row + k + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = (T)a[e]; v[P / 2 + e] = (T)b[e]; }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < P; ++e) v[e] = k + e < kmax ? (T)(float)row[k + e] : (T)0.f;
+  }
+  return __builtin_bit_cast(u32x4, v);
+}
+template <typename T, typename TW, int MB, bool ALIGNED>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(const GemmParams p) {
+  constexpr int P = 16 / sizeof(T), STEP = 4 * P, U = 4;        // k of one matrix instruction group, and how many a turn
+  __shared__ float part[8][MB * 16][16 + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, kg = lane >> 4;
+  const int j0 = blockIdx.x * 16;
+  const T* A = (const T*)p.a;
+  const TW* B = (const TW*)p.b + (int64_t)min(j0 + l16, p.n - 1) * p.ldb;       // columns past n repeat the last one and are not stored
+  const T* rows[MB];
+#pragma unroll
+  for (int u = 0; u < MB; ++u) rows[u] = A + (int64_t)min(u * 16 + l16, p.m - 1) * p.lda;
+  f32x4 acc[MB] = {};
+  for (int64_t k0 = (int64_t)wave * U * STEP; k0 < p.k; k0 += 8 * U * STEP) {
+    u32x4 w[U], x[U][MB];
+#pragma unroll
+    for (int t = 0; t < U; ++t) w[t] = la_piece<T, TW, ALIGNED>(B, k0 + t * STEP + kg * P, p.k);
+#pragma unroll
+    for (int t = 0; t < U; ++t)
+#pragma unroll
+      for (int u = 0; u < MB; ++u) x[t][u] = la_piece<T, T, ALIGNED>(rows[u], k0 + t * STEP + kg * P, p.k);
+#pragma unroll
+    for (int t = 0; t < U; ++t)
+#pragma unroll
+      for (int u = 0; u < MB; ++u) acc[u] = la_mma<T>(w[t], x[t][u], acc[u]);
+  }
+  // acc[u][r]: row 16 u + lane % 16 of C, column 4 (lane / 16) + r
+#pragma unroll
+  for (int u = 0; u < MB; ++u)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[wave][u * 16 + l16][kg * 4 + r] = acc[u][r];
+  __syncthreads();
+  for (int q = threadIdx.x; q < MB * 256; q += 512) {
+    const int i = q >> 4, c = q & 15, j = j0 + c;
+    if (i >= p.m || j >= p.n) continue;
+    float v = part[0][i][c];
+#pragma unroll
+    for (int s = 1; s < 8; ++s) v += part[s][i][c];
+    const float bias = p.bias ? p.bias_f32 ? ((const float*)p.bias)[j] : (float)((const T*)p.bias)[j] : 0.f;
+    la_finish1<T>(p, i, j, v, bias);
+  }
+}
+
 // sums of the splits in their order, and the epilogue
 template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmParams p) {
   const int per = p.ldp / 8;
@@ -517,6 +586,22 @@ static int la_gemm(GemmParams p, LaOperand a, bool ta, LaOperand b, bool tb, int
   return ta ? la_gemm_t<float, true, true>(p, dtype, w, st) : tb ? la_gemm_t<float, false, true>(p, dtype, w, st) : la_gemm_t<float, false, false>(p, dtype, w, st);
 }
 
+// forward of at most 64 rows (a tile of 128 would be half empty and need a second launch to join its splits)
+static const int64_t LA_FEW_ROWS = 64;
+template <typename T, typename TW, int MB> static void la_rows_launch(const GemmParams& p, bool aligned, hipStream_t st) {
+  const dim3 grid((unsigned)vg_ceil_div(p.n, 16));
+  if (aligned) hipLaunchKernelGGL((gemm_rows_kernel<T, TW, MB, true>), grid, dim3(512), 0, st, p);
+  else hipLaunchKernelGGL((gemm_rows_kernel<T, TW, MB, false>), grid, dim3(512), 0, st, p);
+}
+template <typename T, typename TW> static int la_rows(const GemmParams& p, hipStream_t st) {
+  const bool aligned = p.k % (16 / sizeof(T)) == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 && (p.lda * sizeof(T)) % 16 == 0 && (p.ldb * sizeof(TW)) % 16 == 0;
+  if (p.m <= 16) la_rows_launch<T, TW, 1>(p, aligned, st);
+  else if (p.m <= 32) la_rows_launch<T, TW, 2>(p, aligned, st);
+  else la_rows_launch<T, TW, 4>(p, aligned, st);
+  VG_LAUNCH_CHECK();
+  return VG_OK;
+}
+
 static int la_check(const char* what, int64_t m, int64_t n, int64_t k, int act, int dtype) {
   VG_REQUIRE(dtype == VG_F32 || dtype == VG_BF16, "%s: dtype %d", what, dtype);
   VG_REQUIRE(m >= 1 && n >= 1 && k >= 1 && m < (1LL << 30) && n < (1LL << 20) && k < (1LL << 20), "%s: %ld x %ld x %ld", what, (long)m, (long)n, (long)k);
@@ -529,7 +614,7 @@ static int la_weight(const char* what, int w_dtype, int dtype) {
 }
 
 extern "C" size_t vg_linear_act_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype) {
-  return la_ws(m, n, k, dtype, {x, ldx, m, k, 0}, {w, k, n, k, w_dtype == VG_F32});
+  return m <= LA_FEW_ROWS ? 0 : la_ws(m, n, k, dtype, {x, ldx, m, k, 0}, {w, k, n, k, w_dtype == VG_F32});
 }
 extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int w_dtype, const void* bias, int bias_dtype, const void* res,
                                  int64_t ldres, void* y, void* slope, void* ws, int64_t m, int64_t n, int64_t k, int act, int dtype,
@@ -540,6 +625,11 @@ extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int 
   GemmParams p = {};
   p.m = (int)m; p.n = (int)n; p.k = (int)k;
   p.c = y; p.bias = bias; p.bias_f32 = bias_dtype == VG_F32; p.res = res; p.ldres = ldres; p.slope = act == VG_ACT_NONE ? nullptr : slope; p.act = act;
+  if (m <= LA_FEW_ROWS) {
+    p.a = x; p.lda = ldx; p.b = w; p.ldb = k;
+    if (dtype == VG_F32) return la_rows<float, float>(p, (hipStream_t)stream);
+    return w_dtype == VG_F32 ? la_rows<bf16_t, float>(p, (hipStream_t)stream) : la_rows<bf16_t, bf16_t>(p, (hipStream_t)stream);
+  }
   return la_gemm(p, {x, ldx, m, k, 0}, false, {w, k, n, k, w_dtype == VG_F32}, false, dtype, ws, (hipStream_t)stream);
 }
 
