@@ -111,6 +111,28 @@ template <typename T> __device__ __forceinline__ void la_finish1(const GemmParam
   if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j];
   if (p.c_f32) ((float*)p.c)[o] = x; else ((T*)p.c)[o] = (T)x;
 }
+// without an activation
+template <typename T> __device__ __forceinline__ void la_plain8(const GemmParams& p, int i, int j, float* v, const float* bias) {
+  const int64_t o = (int64_t)i * p.n + j;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
+  if (p.vec && j + 8 <= p.n) {
+    if (p.res) {
+      float t[8];
+      get8((const T*)p.res + (int64_t)i * p.ldres + j, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
+    if (p.c_f32) put8((float*)p.c + o, v); else put8((T*)p.c + o, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (j + e < p.n) {
+        const float x = v[e] + (p.res ? (float)((const T*)p.res)[(int64_t)i * p.ldres + j + e] : 0.f);
+        if (p.c_f32) ((float*)p.c)[o + e] = x; else ((T*)p.c)[o + e] = (T)x;
+      }
+  }
+}
 template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v, const float* bias) {
   typedef typename SlopeT<T>::type S;
   const int64_t o = (int64_t)i * p.n + j;
@@ -309,14 +331,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
   }
   la_wait_barrier<0>();                              // the zeros asked for past the end have landed: LDS is free
 
-  // acc[u][v][r] of a lane: row 16 u + lane % 16, column 16 v + 4 (lane / 16) + r.  Through LDS (half of the wave's rows at a
-  // time), so that a lane finishes eight neighbouring columns and a row of the wave's tile leaves as one run of memory.
+  // acc[u][v][r] of a lane: row 16 u + lane % 16, column 16 v + 4 (lane / 16) + r.
+  if (p.part || p.act == VG_ACT_NONE) {
+    // Two neighbouring 16 x 16 blocks exchange rows of lanes, after which a lane has eight neighbouring columns: of the left
+    // block in lanes 0-15 and 32-47, of the right one in the others.
+    const int i1 = i0 + wm * MT * 16 + (lane & 15), j1 = j0 + wn * NT * 16 + ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;
+#pragma unroll
+    for (int v = 0; v < NT; v += 2) {
+      const int j = j1 + v * 16;
+      float bias[8];
+      if (!p.part) la_bias8<T>(p, j, bias);
+#pragma unroll
+      for (int u = 0; u < MT; ++u) {
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[u][v][r]), __float_as_uint(acc[u][v + 1][r]), false, false);
+          x[r] = __uint_as_float(s[0]);
+          x[4 + r] = __uint_as_float(s[1]);
+        }
+        const int i = i1 + u * 16;
+        if (i < p.m && j < p.n) {
+          if (p.part) put8(p.part + ((int64_t)split * p.m + i) * p.ldp + j, x);
+          else la_plain8<T>(p, i, j, x, bias);
+        }
+      }
+    }
+    return;
+  }
+  // With an activation: through LDS (half of the wave's rows at a time) into a loop, since sixteen copies of the activations
+  // would not stay in the instruction cache.
   constexpr int LDW = 16 * NT + 4, HALF = MT / 2;
   static_assert(64 % (2 * NT) == 0, "a lane keeps its columns");
   float* st = (float*)smem + wave * 16 * HALF * LDW;
   const int c = (lane % (2 * NT)) * 8, j = j0 + wn * NT * 16 + c;
   float bias[8];
-  if (!p.part) la_bias8<T>(p, j, bias);
+  la_bias8<T>(p, j, bias);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -333,10 +383,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
       float v[8];
       *(f32x4*)v = *(const f32x4*)(st + r * LDW + c);
       *(f32x4*)(v + 4) = *(const f32x4*)(st + r * LDW + c + 4);
-      if (i < p.m && j < p.n) {
-        if (p.part) put8(p.part + ((int64_t)split * p.m + i) * p.ldp + j, v);
-        else la_finish8<T>(p, i, j, v, bias);
-      }
+      if (i < p.m && j < p.n) la_finish8<T>(p, i, j, v, bias);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
