@@ -211,7 +211,10 @@ template <typename T, bool TR, int R, int NTH, int KB> struct LaTile {
       }
     }
   }
-  static __device__ __forceinline__ int swz(int k) { return EB == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3; }
+  static __device__ __forceinline__ int swz(int k) {
+    if (EB == 4) return (k >> 2) & 3;
+    return RB == 128 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;      // a 128-byte row is half the banks
+  }
   // k0: first k of the tile; klimit: pieces at or beyond it come as zeros
   __device__ __forceinline__ void load(int i, la_srd_t srd, unsigned lds, int wave, int k0, int klimit) const {
     la_dma16(srd, k0 + kof[i] < klimit ? voff[i] : 0xFFFFFFFFu, lds + (i * NTH + wave * 64) * 16);
@@ -224,7 +227,7 @@ template <typename T, bool TR, int R, int NTH, int KB> struct LaTile {
       return *(const u32x4*)(s + r * KB + (((ks * 4 + kg) ^ turn(r)) << 4));
     } else if constexpr (EB == 2) {
       const int tq = l16 >> 2, tp = l16 & 3, k = ks * 32 + kg * 8 + tq;
-      const unsigned char* a = s + k * RB + ((tile ^ (tq | (kg & 1) << 2)) << 5) + tp * 8;
+      const unsigned char* a = s + k * RB + ((tile ^ swz(k)) << 5) + tp * 8;
       const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_tr_t)a);
       const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_tr_t)(a + 4 * RB));
       return __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
@@ -474,11 +477,19 @@ template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(co
   la_finish8<T>(p, i, j, v, bias);
 }
 
-// [rows][cols] (row stride ld) into [rows][pitch], the padding zeroed; S -> T rounds (an f32 master weight for bf16 products)
+// Matrices [rows][cols] (row stride ld) into [rows][pitch], the padding zeroed: both operands of a product in one launch, the
+// first taking `split` blocks.  f32 sources of bf16 products (master weights) are rounded.
+struct PackParams {
+  const void* src[2];
+  void* dst[2];
+  int64_t ld[2], rows[2];
+  int cols[2], pitch[2], f32[2];
+  unsigned split;
+};
 template <typename S, typename T>
-__global__ __launch_bounds__(256) void la_pack_kernel(const S* __restrict__ src, int64_t ld, T* __restrict__ dst, int64_t rows, int cols, int pitch) {
+__device__ __forceinline__ void la_pack_one(const S* src, int64_t ld, T* dst, int64_t rows, int cols, int pitch, int64_t block, int64_t blocks) {
   const int per = pitch / 8;
-  for (int64_t q = blockIdx.x * (int64_t)256 + threadIdx.x; q < rows * per; q += (int64_t)gridDim.x * 256) {
+  for (int64_t q = block * 256 + threadIdx.x; q < rows * per; q += blocks * 256) {
     const int64_t r = q / per;
     const int c = (int)(q % per) * 8;
     float v[8];
@@ -486,6 +497,12 @@ __global__ __launch_bounds__(256) void la_pack_kernel(const S* __restrict__ src,
     for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)src[r * ld + c + e] : 0.f;
     put8(dst + r * pitch + c, v);
   }
+}
+template <typename T> __global__ __launch_bounds__(256) void la_pack_kernel(const PackParams p) {
+  const int w = blockIdx.x >= p.split;
+  const int64_t block = w ? blockIdx.x - p.split : blockIdx.x, blocks = w ? gridDim.x - p.split : p.split;
+  if (sizeof(T) == 2 && p.f32[w]) la_pack_one((const float*)p.src[w], p.ld[w], (T*)p.dst[w], p.rows[w], p.cols[w], p.pitch[w], block, blocks);
+  else la_pack_one((const T*)p.src[w], p.ld[w], (T*)p.dst[w], p.rows[w], p.cols[w], p.pitch[w], block, blocks);
 }
 
 // dz = dy slope (dz = dy without one) and partial column sums of the unrounded dz: part[row chunk][n].
@@ -543,24 +560,30 @@ static bool la_direct(const LaOperand& o, int dtype) {
 }
 static size_t la_packed_bytes(const LaOperand& o, int dtype) { return la_up((size_t)o.rows * la_pitch(o.cols) * vg_elt_size(dtype)); }
 
-// Which tiles, and how many ways the contraction is split (partial sums in f32, joined by a kernel): the cheapest by
-//   rounds of blocks over the chip * (128-byte steps of k * step + fixed)  +  traffic and launch of the join
-// with the measured times (us) of a step and of a block's ends: 256 x 256 (one block a CU) 1.7 and 7, 128 x 128 (two) 1.15 and 5,
-// f32 128 x 128 4.1 and 5.  E.g. dW of 16384 x 1024 x 4096: 128 x 128 in two parts 187 us, 256 x 256 in four 158.
-struct LaPlan { int big, splits, ktiles; };
+// Which tiles, and how many ways the contraction is split (partial sums in f32, joined by a kernel): the cheapest by an estimate
+// from measured times (us).  A CU with nb blocks takes max(lat, nb * step) for 128 bytes of k of each, and `fixed` for the ends
+// of every `res` blocks that it holds at once; a join costs its launch and the partial sums' way out and back.
+//   tile    bf16 lat  step  fixed  res     f32 lat  step  fixed
+//   64          0.26  0.20   2.5    3         0.6   0.53   3.0
+//   128         0.68  0.55   3.5    2         2.0   2.0    5.0
+//   256         1.50  1.65   6.0    1
+// E.g. bf16 1024^3: 64 unsplit 6.9, 128 unsplit 12.1, 128 in eight 25; dW of 16384 x 1024 x 4096: 256 in four 145, 128 in two 187;
+// forward of 16381 x 2048 x 512: 128 39, 256 57.
+struct LaPlan { int tile, splits, ktiles; double us; };
 static LaPlan la_plan(int64_t m, int64_t n, int64_t k, int dtype) {
+  struct Cost { int tile, res; double lat, step, fixed; };
+  static const Cost bf16[3] = {{64, 3, 0.26, 0.20, 2.5}, {128, 2, 0.68, 0.55, 3.5}, {256, 1, 1.50, 1.65, 6.0}};
+  static const Cost f32[2] = {{64, 3, 0.6, 0.53, 3.0}, {128, 2, 2.0, 2.0, 5.0}};
   const int64_t kt = vg_ceil_div(k * vg_elt_size(dtype), 128);
-  LaPlan best = {0, 1, (int)kt};
-  double least = 1e30;
-  for (int big = 0; big <= (dtype == VG_BF16 ? 1 : 0); ++big) {
-    const int64_t tiles = big ? vg_ceil_div(m, 256) * vg_ceil_div(n, 256) : vg_ceil_div(m, 128) * vg_ceil_div(n, 128);
-    const int64_t slots = big ? 256 : 512;
-    const double step = dtype == VG_F32 ? 4.1 : big ? 1.7 : 1.15, fixed = big ? 7 : 5;
+  LaPlan best = {64, 1, (int)kt, 1e30};
+  for (int i = 0; i < (dtype == VG_BF16 ? 3 : 2); ++i) {
+    const Cost& c = dtype == VG_BF16 ? bf16[i] : f32[i];
+    const int64_t tiles = vg_ceil_div(m, c.tile) * vg_ceil_div(n, c.tile);
     for (int64_t s = 1; s <= 32 && (s == 1 || kt / s >= 4); s += s < 4 ? 1 : s < 8 ? 2 : 4) {
-      const int64_t per = vg_ceil_div(kt, s), parts = vg_ceil_div(kt, per);
-      const double join = parts > 1 ? 4 + (double)parts * m * n * 8 / 4.5e6 : 0;
-      const double t = vg_ceil_div(tiles * parts, slots) * (per * step + fixed) + join;
-      if (t < least) { least = t; best = {big, (int)parts, (int)per}; }
+      const int64_t per = vg_ceil_div(kt, s), parts = vg_ceil_div(kt, per), nb = vg_ceil_div(tiles * parts, 256);
+      const double join = parts > 1 ? 4.5 + (double)parts * m * n * 1.07e-6 : 0;
+      const double us = per * (nb * c.step > c.lat ? nb * c.step : c.lat) + c.fixed * vg_ceil_div(nb, c.res) + join;
+      if (us < best.us) best = {c.tile, (int)parts, (int)per, us};
     }
   }
   return best;
@@ -573,21 +596,26 @@ static size_t la_ws(int64_t m, int64_t n, int64_t k, int dtype, const LaOperand&
   return la_part_bytes(m, n, k, dtype) + (la_direct(a, dtype) ? 0 : la_packed_bytes(a, dtype)) + (la_direct(b, dtype) ? 0 : la_packed_bytes(b, dtype));
 }
 
-template <typename S, typename T> static void la_pack_launch(const LaOperand& o, void* dst, hipStream_t st) {
-  const int pitch = (int)la_pitch(o.cols);
-  int64_t blocks = vg_ceil_div(o.rows * (pitch / 8), 256);
-  if (blocks > 8192) blocks = 8192;
-  hipLaunchKernelGGL((la_pack_kernel<S, T>), dim3((unsigned)blocks), dim3(256), 0, st, (const S*)o.p, o.ld, (T*)dst, o.rows, (int)o.cols, pitch);
-}
-static char* la_pack(LaOperand* o, int dtype, char* ws, hipStream_t st) {
-  if (la_direct(*o, dtype)) return ws;
-  if (dtype == VG_F32) la_pack_launch<float, float>(*o, ws, st);
-  else if (o->src_f32) la_pack_launch<float, bf16_t>(*o, ws, st);
-  else la_pack_launch<bf16_t, bf16_t>(*o, ws, st);
-  const size_t n = la_packed_bytes(*o, dtype);
-  o->p = ws;
-  o->ld = la_pitch(o->cols);
-  return ws + n;
+// copies what the tiles cannot read in place to the workspace; returns its first free byte
+static char* la_pack(LaOperand* o[2], int dtype, char* ws, hipStream_t st) {
+  PackParams p = {};
+  unsigned blocks[2] = {0, 0};
+  int n = 0;
+  for (int i = 0; i < 2; ++i) {
+    if (la_direct(*o[i], dtype)) continue;
+    const int64_t pitch = la_pitch(o[i]->cols), need = vg_ceil_div(o[i]->rows * (pitch / 8), 256);
+    p.src[n] = o[i]->p; p.dst[n] = ws; p.ld[n] = o[i]->ld; p.rows[n] = o[i]->rows; p.cols[n] = (int)o[i]->cols; p.pitch[n] = (int)pitch; p.f32[n] = o[i]->src_f32;
+    blocks[n++] = (unsigned)(need < 8192 ? need : 8192);
+    const size_t bytes = la_packed_bytes(*o[i], dtype);
+    o[i]->p = ws; o[i]->ld = pitch;
+    ws += bytes;
+  }
+  if (n) {
+    p.split = blocks[0];
+    if (dtype == VG_BF16) hipLaunchKernelGGL(la_pack_kernel<bf16_t>, dim3(blocks[0] + blocks[1]), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(la_pack_kernel<float>, dim3(blocks[0] + blocks[1]), dim3(256), 0, st, p);
+  }
+  return ws;
 }
 
 template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S, int KB> static int la_tile_launch(GemmParams p, hipStream_t st) {
@@ -609,8 +637,12 @@ template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int d
   p.ldp = (int)la_pitch(p.n);
   p.part = pl.splits > 1 ? (float*)ws : nullptr;
   int rc;
-  if constexpr (sizeof(T) == 2) rc = pl.big ? la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2, 128>(p, st) : la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2, 128>(p, st);
-  else rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2, 128>(p, st);       // bound by the f32 matrix rate at either size
+  if (pl.tile == 64) rc = la_tile_launch<T, TA, TB, 2, 2, 2, 2, 3, 128>(p, st);
+  else if (pl.tile == 128) rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2, 128>(p, st);
+  else {
+    if constexpr (sizeof(T) == 2) rc = la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2, 128>(p, st);
+    else rc = VG_ERR_UNSUPPORTED;                    // not planned for f32, whose matrix rate binds at any size
+  }
   if (rc) return rc;
   if (pl.splits > 1) {
     hipLaunchKernelGGL(gemm_join_kernel<T>, dim3((unsigned)vg_ceil_div((int64_t)p.m * (p.ldp / 8), 256)), dim3(256), 0, st, p);
@@ -622,8 +654,8 @@ template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int d
 static int la_gemm(GemmParams p, LaOperand a, bool ta, LaOperand b, bool tb, int dtype, void* ws, hipStream_t st) {
   VG_REQUIRE((uintptr_t)ws % 256 == 0 && (ws || la_ws(p.m, p.n, p.k, dtype, a, b) == 0), "linear_act: needs a workspace, aligned to 256 bytes");
   const int e = vg_elt_size(dtype);
-  char* w = la_pack(&a, dtype, (char*)ws, st);
-  w = la_pack(&b, dtype, w, st);
+  LaOperand* both[2] = {&a, &b};
+  char* w = la_pack(both, dtype, (char*)ws, st);
   VG_LAUNCH_CHECK();
   p.a = a.p; p.lda = a.ld; p.b = b.p; p.ldb = b.ld;
   auto al = [](const void* q) { return (uintptr_t)q % 16 == 0; };
@@ -633,8 +665,20 @@ static int la_gemm(GemmParams p, LaOperand a, bool ta, LaOperand b, bool tb, int
   return ta ? la_gemm_t<float, true, true>(p, dtype, w, st) : tb ? la_gemm_t<float, false, true>(p, dtype, w, st) : la_gemm_t<float, false, false>(p, dtype, w, st);
 }
 
-// forward of at most 64 rows (a tile of 128 would be half empty and need a second launch to join its splits)
-static const int64_t LA_FEW_ROWS = 64;
+// Whether the few-rows kernel takes a forward product: its time is bound by one read of the weights from memory (3.9 TB/s) or
+// by every block's read of x from the cache (7 TB/s), against the tiles' and the copies that they need of f32 master weights
+// or of rows that are not whole 16-byte pieces.  bf16 64 x 1024 x 4096: 8.0 us here, 6.7 in tiles; 32 rows: 5.7 and 6.7; 64
+// rows with f32 weights: 9.1 and 25.
+static bool la_few_rows(int64_t m, int64_t n, int64_t k, int dtype, const LaOperand& x, const LaOperand& w) {
+  if (m > 64) return false;
+  const double e = vg_elt_size(dtype), ew = w.src_f32 ? 4 : e;
+  const double read = n * (double)k * ew / 3.9e6, cached = vg_ceil_div(n, 16) * (double)m * k * e / 7e6;
+  const double few = 2.5 + (read > cached ? read : cached);
+  double tiles = la_plan(m, n, k, dtype).us;
+  if (!la_direct(w, dtype)) tiles += 3 + n * (double)k * (ew + e) / 4e6;
+  if (!la_direct(x, dtype)) tiles += 3;
+  return few <= tiles;
+}
 template <typename T, typename TW, int MB> static void la_rows_launch(const GemmParams& p, bool aligned, hipStream_t st) {
   const dim3 grid((unsigned)vg_ceil_div(p.n, 16));
   if (aligned) hipLaunchKernelGGL((gemm_rows_kernel<T, TW, MB, true>), grid, dim3(512), 0, st, p);
@@ -661,7 +705,8 @@ static int la_weight(const char* what, int w_dtype, int dtype) {
 }
 
 extern "C" size_t vg_linear_act_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype) {
-  return m <= LA_FEW_ROWS ? 0 : la_ws(m, n, k, dtype, {x, ldx, m, k, 0}, {w, k, n, k, w_dtype == VG_F32});
+  const LaOperand a = {x, ldx, m, k, 0}, b = {w, k, n, k, w_dtype == VG_F32};
+  return la_few_rows(m, n, k, dtype, a, b) ? 0 : la_ws(m, n, k, dtype, a, b);
 }
 extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int w_dtype, const void* bias, int bias_dtype, const void* res,
                                  int64_t ldres, void* y, void* slope, void* ws, int64_t m, int64_t n, int64_t k, int act, int dtype,
@@ -672,12 +717,13 @@ extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int 
   GemmParams p = {};
   p.m = (int)m; p.n = (int)n; p.k = (int)k;
   p.c = y; p.bias = bias; p.bias_f32 = bias_dtype == VG_F32; p.res = res; p.ldres = ldres; p.slope = act == VG_ACT_NONE ? nullptr : slope; p.act = act;
-  if (m <= LA_FEW_ROWS) {
+  const LaOperand a = {x, ldx, m, k, 0}, b = {w, k, n, k, w_dtype == VG_F32};
+  if (la_few_rows(m, n, k, dtype, a, b)) {
     p.a = x; p.lda = ldx; p.b = w; p.ldb = k;
     if (dtype == VG_F32) return la_rows<float, float>(p, (hipStream_t)stream);
     return w_dtype == VG_F32 ? la_rows<bf16_t, float>(p, (hipStream_t)stream) : la_rows<bf16_t, bf16_t>(p, (hipStream_t)stream);
   }
-  return la_gemm(p, {x, ldx, m, k, 0}, false, {w, k, n, k, w_dtype == VG_F32}, false, dtype, ws, (hipStream_t)stream);
+  return la_gemm(p, a, false, b, false, dtype, ws, (hipStream_t)stream);
 }
 
 // chunks of rows: enough blocks to fill the chip, at least 32 rows each so that the partial sums stay a small part of the traffic
