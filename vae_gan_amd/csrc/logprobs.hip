@@ -88,22 +88,34 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k)
   return ((unsigned long long)hi << 32) | lo;
 }
 
-// the `top` largest of n different keys, to put(k, key), by one wave
+// the `top` largest of n different keys (0: none), to put(k, key), by one wave
 template <typename F> __device__ __forceinline__ void best_of(const unsigned long long* keys, int n, int top, int lane, F put) {
   if (n <= 64) {                                     // each lane counts the keys above its own
     const unsigned long long mine = lane < n ? keys[lane] : 0;
     int above = 0;
-    for (int q = 0; q < n; ++q) above += keys[q] > mine;
-    if (lane < n && mine && above < top) put(above, mine);
+    for (int q = 0; q < n; ++q) {
+      const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), q) << 32 |
+                                   (unsigned)__builtin_amdgcn_readlane((int)mine, q);
+      above += o > mine;
+    }
+    if (mine && above < top) put(above, mine);
     return;
   }
+  constexpr int R = 8;                               // the first 512 in registers
+  unsigned long long mine[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) mine[r] = r * 64 + lane < n ? keys[r * 64 + lane] : 0;
   unsigned long long last = ~0ull;
   for (int k = 0; k < top; ++k) {
     unsigned long long b = 0;
-    for (int q = lane; q < n; q += 64)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (mine[r] < last && mine[r] > b) b = mine[r];
+    for (int q = R * 64 + lane; q < n; q += 64)
       if (keys[q] < last && keys[q] > b) b = keys[q];
     last = wave_max_key(b);
-    if (lane == 0) put(k, last);
+    if (lane == 0 && last) put(k, last);
+    if (!last) break;
   }
 }
 
@@ -345,26 +357,40 @@ __global__ __launch_bounds__(256) void lp_row_kernel(const LpParams p) {
   if (p.top) lp_best<T, TEAM>(p, u, lists[threadIdx.x / TEAM], mine, a);
 }
 
-// the splits of one row
-#define LP_JOIN 2048
+// The splits of one row.  Its parts (memory, selection, sums) run side by side on the block's waves: each wave takes a quarter
+// of the splits' best, the last wave fetches the token's logit meanwhile.
 template <typename T> __global__ __launch_bounds__(256) void lp_join_kernel(const LpParams p) {
-  __shared__ unsigned long long keys[LP_JOIN];
-  const int lane = threadIdx.x & 63, n = p.splits * p.top;
+  __shared__ unsigned long long some[4 * LP_MAX_TOP], win[LP_MAX_TOP];
+  __shared__ float sums[3], xt;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = p.splits * p.top;
   const int64_t row = blockIdx.x;
-  const unsigned long long* c = p.cand + row * n;
-  if (n <= LP_JOIN) {
-    for (int q = threadIdx.x; q < n; q += 256) keys[q] = c[q];
-    __syncthreads();
+  if (threadIdx.x == 255) xt = token_logit<T>(p, row);
+  if (p.top) {
+    const int per = (n + 3) / 4, lo = wave * per < n ? wave * per : n, hi = lo + per < n ? lo + per : n;
+    if (lane < p.top) some[wave * p.top + lane] = 0;          // a quarter may hold fewer
+    __builtin_amdgcn_wave_barrier();
+    best_of(p.cand + row * n + lo, hi - lo, p.top, lane, [&](int k, unsigned long long key) { some[wave * p.top + k] = key; });
   }
-  if (threadIdx.x >= 64) return;
-  Soft a = {-__builtin_inff(), 0.f, 0.f};
-  for (int s = lane; s < p.splits; s += 64) {
-    const float* o = p.part + (row * p.splits + s) * 4;
-    a = soft_join(a, Soft{o[0], o[1], o[2]});
+  if (wave == 0) {
+    Soft a = {-__builtin_inff(), 0.f, 0.f};
+    for (int s = lane; s < p.splits; s += 64) {
+      const f32x4 o = *(const f32x4*)(p.part + (row * p.splits + s) * 4);
+      a = soft_join(a, Soft{o[0], o[1], o[2]});
+    }
+    a = soft_wave(a);
+    if (lane == 0) { sums[0] = a.m; sums[1] = a.s; sums[2] = a.u; }
   }
-  a = soft_wave(a);
-  if (lane == 0) finish_row(p, row, a, token_logit<T>(p, row));
-  if (p.top) best_of(n <= LP_JOIN ? keys : c, n, p.top, lane, [&](int k, unsigned long long key) { put_top(p, row, k, key, a); });
+  __syncthreads();
+  const Soft a = {sums[0], sums[1], sums[2]};
+  if (threadIdx.x == 64) finish_row(p, row, a, xt);
+  if (!p.top) return;
+  if (wave == 0) {
+    best_of(some, 4 * p.top, p.top, lane, [&](int k, unsigned long long key) { win[k] = key; });
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (lane < p.top) put_top(p, row, lane, win[lane], a);
+  }
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
@@ -438,11 +464,12 @@ static int lp_check(const char* what, int64_t rows, int vocab, int64_t ldx, int 
 }
 static bool lp_regs(int vocab) { return vocab <= 64 * 32; }      // a row in the registers of a wave
 
+static size_t lp_keys_bytes(int64_t rows, int splits, int top) { return ((size_t)rows * splits * top * 8 + 15) / 16 * 16; }
 extern "C" size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top) {
   if (rows <= 0 || vocab <= 0 || lp_regs(vocab)) return 0;
   int s, c;
   lp_split(rows, vocab, &s, &c);
-  return s == 1 ? 0 : (size_t)rows * s * (4 * sizeof(float) + (size_t)top * 8);
+  return s == 1 ? 0 : (size_t)rows * s * 4 * sizeof(float) + lp_keys_bytes(rows, s, top);
 }
 
 static const int64_t LP_WAVE_UNITS = 2048;          // two waves a SIMD
@@ -477,11 +504,12 @@ extern "C" int vg_token_logprobs_fwd(const void* logits, int64_t ldx, const int6
   if (int rc = lp_check("token_logprobs_fwd", rows, vocab, ldx, top, dtype)) return rc;
   if (rows == 0) return VG_OK;
   VG_REQUIRE(logits && tokens && logp && entropy && (!top || (top_logp && top_at)), "token_logprobs_fwd: null pointer");
-  VG_REQUIRE(ws || vg_token_logprobs_ws_bytes(rows, vocab, top) == 0, "token_logprobs_fwd: needs a workspace");
+  VG_REQUIRE((uintptr_t)ws % 16 == 0 && (ws || vg_token_logprobs_ws_bytes(rows, vocab, top) == 0),
+             "token_logprobs_fwd: needs a workspace, aligned to 16 bytes");
   LpParams p = {logits, ldx, tokens, ignore, rows, vocab, top, 1, 0, logp, entropy, lse, top_logp, top_at, nullptr, nullptr};
   lp_split(rows, vocab, &p.splits, &p.chunk);
   p.cand = (unsigned long long*)ws;                  // 8-byte values first
-  p.part = (float*)((char*)ws + (size_t)rows * p.splits * top * 8);
+  p.part = (float*)((char*)ws + lp_keys_bytes(rows, p.splits, top));
   if (dtype == VG_BF16) lp_launch<bf16_t>(p, (hipStream_t)stream);
   else lp_launch<float>(p, (hipStream_t)stream);
   VG_LAUNCH_CHECK();
