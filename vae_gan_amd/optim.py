@@ -119,7 +119,10 @@ class FlatAdamW(FlatAdam):
     ``state_bits=8``: the moments take 2 bytes a parameter instead of 8.  Every 256 elements of a tensor share one f32 scale for
     ``exp_avg`` and one for ``root_sq`` (the root of the second moment; half the dynamic range of the moment itself), kept as
     e4m3 values (``exp_avg * exp_avg_scale``).  A step uses this step's moments before they are rounded.  An element whose
-    gradient is not finite keeps NaN moments, as it would in 32 bits; the rest of its 256 is not touched."""
+    gradient is not finite keeps NaN moments, as it would in 32 bits; the rest of its 256 is not touched.
+
+    ``load_state_dict`` takes the hyperparameters of the file, as torch does: a ``FlatAdam`` file (32 bits) brings a weight
+    decay of 0.  8- and 32-bit states are not converted into each other (ValueError)."""
 
     ALIGN = 256         # elements that share a scale (csrc/adamw.hip)
 
@@ -147,18 +150,21 @@ class FlatAdamW(FlatAdam):
         self.exp_avg_scale = torch.zeros(n // self.ALIGN, dtype=torch.float32, device=dev)
         self.root_sq_scale = torch.zeros(n // self.ALIGN, dtype=torch.float32, device=dev)
 
+    def step(self, grad_scale: float = 1.0):
+        with ops._on_device("adamw_step", self.flat_p):      # the update and the re-packed weight images
+            super().step(grad_scale)
+
     def _update(self, grad_scale: float):
         lib = L.load()
         tail = (L.ptr(self._decay), self.numel, self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.step_count,
                 grad_scale)
-        with ops._on_device("adamw_step", self.flat_p):
-            if self.state_bits == 32:
-                L.check(lib.vg_adamw_step(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.exp_avg.data_ptr(),
-                                          self.exp_avg_sq.data_ptr(), *tail, L.stream()), "adamw_step")
-            else:
-                L.check(lib.vg_adamw8_step(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.exp_avg.data_ptr(),
-                                           self.exp_avg_scale.data_ptr(), self.root_sq.data_ptr(), self.root_sq_scale.data_ptr(),
-                                           *tail, L.stream()), "adamw8_step")
+        if self.state_bits == 32:
+            L.check(lib.vg_adamw_step(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.exp_avg.data_ptr(),
+                                      self.exp_avg_sq.data_ptr(), *tail, L.stream()), "adamw_step")
+        else:
+            L.check(lib.vg_adamw8_step(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.exp_avg.data_ptr(),
+                                       self.exp_avg_scale.data_ptr(), self.root_sq.data_ptr(), self.root_sq_scale.data_ptr(),
+                                       *tail, L.stream()), "adamw8_step")
 
     @property
     def param_groups(self):
