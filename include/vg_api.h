@@ -416,6 +416,10 @@ size_t vg_linear_act_wgrad_ws_bytes(const void* dz, const void* x, int64_t ldx, 
 int vg_linear_act_wgrad(const void* dz, const void* x, int64_t ldx, void* dw, int dw_dtype, void* ws, int64_t m, int64_t n, int64_t k,
                         int dtype, void* stream);
 
+/* Name of the kernel variant that the calling thread's last vg_linear_act_fwd / _dgrad / _wgrad launched ("rows<bf16,16>",
+ * "tile<bf16,256,nt>+join": tile size, n / t per operand for the layouts, + join where the contraction was split). */
+const char* vg_last_linear_act_kernel(void);
+
 /* Log probability of tokens[r] under row r of logits [rows][vocab] (row stride ldx), the row's entropy (nats) and its `top` best
  * alternatives (0..32; by value, then by lower place).  lse: [rows][2] f32 out for the backward pass (the row's maximum and log2 of its sum), or NULL.  -inf logits are
  * masked; a row of only -inf gives logp -inf, entropy 0, gradient 0; NaN or +inf in a row gives NaN (a NaN ranks as -inf among the

@@ -324,6 +324,101 @@ def test_linear_act_nonfinite_values_stay_in_their_rows(dt):
     assert not big.isnan().any() and float(big.abs().max()) == 0                # e^80000 overflows: the limit is 0
 
 
+def test_linear_act_kernel_variants():
+    """Every tile size, unsplit and split, in each product's layout, and the few-rows kernels, against f64 through the C ABI."""
+    from vae_gan_amd import lib as L
+    lib = L.load()
+    P = lambda t: t.data_ptr()      # noqa: E731
+    seen = set()
+
+    def note(out, ref, tol):
+        seen.add(lib.vg_last_linear_act_kernel().decode())
+        within(out, ref, tol, lib.vg_last_linear_act_kernel().decode())
+    for dt, shapes in ((BF16, [(16384, 1024, 4096), (16300, 1000, 4090), (4096, 256, 4096), (4096, 1024, 256), (4096, 4096, 256), (1024, 512, 512), (300, 4096, 300),
+                               (1000, 264, 2000), (4000, 128, 128), (64, 256, 2048), (16, 64, 64), (30, 64, 64), (700, 8192, 1400), (16384, 512, 2048),
+                               (2048, 128, 2048), (128, 2048, 2048), (768, 4096, 1536), (768, 1536, 4096), (1536, 8192, 1536), (1536, 1536, 8192)]),
+                       (F32, [(4096, 512, 2048), (2048, 2048, 512), (1024, 512, 512), (300, 4096, 300), (4000, 128, 128), (16, 64, 64), (30, 64, 64), (64, 64, 64),
+                              (16384, 256, 1024), (300, 300, 4096), (2048, 128, 2048), (2048, 2048, 128), (128, 2048, 2048), (768, 1024, 1536),
+                              (768, 1536, 1024), (1024, 768, 1536)])):
+        code, e = L.vg_dtype(dt), half(dt)
+        for m, k, n in shapes:
+            g = gen(m + k + n)
+            x, w, dz = (torch.randn(*s_, device="cuda", generator=g).to(dt) for s_ in ((m, k), (n, k), (m, n)))
+            X, W, Z = x.double(), w.double(), dz.double()
+            y, dx, dw = torch.empty(m, n, dtype=dt, device="cuda"), torch.empty_like(x), torch.empty_like(w)
+            ws = torch.empty(max(lib.vg_linear_act_fwd_ws_bytes(P(x), k, P(w), code, m, n, k, code), lib.vg_linear_act_dgrad_ws_bytes(P(dz), P(w), code, m, n, k, code),
+                                 lib.vg_linear_act_wgrad_ws_bytes(P(dz), P(x), k, m, n, k, code), 1), dtype=torch.uint8, device="cuda")
+            L.check(lib.vg_linear_act_fwd(P(x), k, P(w), code, None, 0, None, 0, P(y), None, P(ws), m, n, k, 0, code, L.stream()))
+            ref = X @ W.t()
+            note(y, ref, e * ref.abs() + (k + 4) * U * (X.abs() @ W.abs().t()))
+            L.check(lib.vg_linear_act_dgrad(P(dz), P(w), code, P(dx), P(ws), m, n, k, code, L.stream()))
+            ref = Z @ W
+            note(dx, ref, e * ref.abs() + (n + 4) * U * (Z.abs() @ W.abs()))
+            L.check(lib.vg_linear_act_wgrad(P(dz), P(x), k, P(dw), code, P(ws), m, n, k, code, L.stream()))
+            ref = Z.t() @ X
+            note(dw, ref, e * ref.abs() + (m + 4) * U * (Z.t().abs() @ X.abs()))
+    want = {f"rows<{t},{r}>" for t in ("bf16", "f32") for r in (16, 32, 64)}
+    want |= {f"tile<{t},{size},{layout}>{join}" for t, size in (("bf16", 64), ("bf16", 128), ("bf16", 256), ("f32", 64), ("f32", 128))
+             for layout in ("nn", "nt", "tt") for join in ("", "+join")}
+    assert want <= seen, (sorted(want - seen), sorted(seen))
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_linear_act_rows_far_apart(dt):
+    """Rows 10 MB and more apart: beyond what a tile's 32-bit offsets cover, so they are copied first."""
+    _, w, b, res, dy = la_data(150, 64, 72, dt, 37)
+    wide = torch.empty(150, 5_000_000 if dt == BF16 else 2_600_000, dtype=dt, device="cuda")
+    wide[:, :64] = torch.randn(150, 64, device="cuda", generator=gen(2)).to(dt)
+    la_check(wide[:, :64], w, b, "silu", res, dy)
+    la_check(wide[:7, :64], w, b, "none", None, dy[:7])
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements and 2^32 bytes in one tensor: the first and the last rows against f64."""
+    from vae_gan_amd import lib as L
+    from vae_gan_amd import ops
+    rows, c = 70000, 32768
+    x = torch.empty(rows, c, dtype=BF16, device="cuda")
+    ends = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    x[ends] = torch.randn(5, c, device="cuda", generator=gen(6)).to(BF16)
+    w, b = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    with torch.no_grad():
+        y = ops.layer_norm(x, w, b)
+        ref = ln_oracle(x[ends], w, b, None, c, 1e-5, BF16)
+        within(y[ends], *ref["y"], "layer norm")
+        del y
+        t = torch.randint(0, c, (rows,), device="cuda", generator=gen(7))
+        logp, ent, _, _ = ops.token_logprobs(x, t)
+        ref, _ = lp_oracle(x[ends].double(), t[ends], None, None, -100, BF16)
+        within(logp[ends], *ref["logp"], "logp")
+        within(ent[ends], *ref["entropy"], "entropy")
+    xg = x.requires_grad_()
+    out = ops.token_logprobs(xg, t)
+    da, db = torch.randn(rows, device="cuda", generator=gen(8)), torch.randn(rows, device="cuda", generator=gen(9))
+    (dx,) = torch.autograd.grad(out[:2], (xg,), (da, db))
+    ref, _ = lp_oracle(x[ends].detach().double(), t[ends], da[ends], db[ends], -100, BF16)
+    within(dx[ends], *ref["dx"], "dlogits")
+    del dx, out, xg, x
+    m, k, n = 70000, 16, 32768
+    a, wt = torch.randn(m, k, device="cuda", generator=gen(1)).to(BF16), torch.randn(n, k, device="cuda", generator=gen(2)).to(BF16)
+    ends = torch.tensor([0, 63, m - 65, m - 1], device="cuda")
+    with torch.no_grad():
+        y = ops.linear_act(a, wt, None, L.ACT_LRELU)
+    ref = la_oracle(a[ends], wt, None, None, None, "lrelu", BF16)
+    within(y[ends], *ref["y"], "linear_act")
+    # the same tensor as the input of a product: contraction over its 70000 rows, and over its 32768 columns
+    with torch.no_grad():
+        z = ops.linear_act(y, torch.ones(8, n, dtype=BF16, device="cuda"))
+    want = y[ends].double().sum(1, keepdim=True).expand(-1, 8)
+    within(z[ends], want, half(BF16) * want.abs() + (n + 4) * U * y[ends].double().abs().sum(1, keepdim=True), "wide rows")
+    wg = torch.zeros(8, n, dtype=BF16, device="cuda", requires_grad=True)
+    dz = torch.zeros(m, 8, dtype=BF16, device="cuda")
+    dz[ends] = 1
+    (dw,) = torch.autograd.grad(ops.linear_act(y, wg), (wg,), dz)
+    want = y[ends].double().sum(0, keepdim=True).expand(8, -1)
+    within(dw, want, half(BF16) * want.abs() + 8 * U * y[ends].double().abs().sum(0, keepdim=True), "long contraction")
+
+
 def test_linear_act_gradient_against_differences():
     g = gen(8)
     x, w, b = (torch.randn(*s, device="cuda", generator=g) for s in ((3, 9), (5, 9), (5,)))
@@ -406,7 +501,7 @@ def lp_check(x, t, top=0, ignore=-100, seed=0):
     return logp.detach(), ent.detach(), tl, ta, dx
 
 
-LP_SHAPES = [(1, 1, 0), (3, 2, 0), (5, 8, 0), (9, 63, 1), (130, 64, 0), (7, 100, 4), (64, 512, 0), (31, 513, 0), (3, 1000, 24), (17, 2048, 0), (9, 2049, 0),
+LP_SHAPES = [(2100, 2500, 3), (2050, 5001, 0), (2200, 4096, 0), (1, 1, 0), (3, 2, 0), (5, 8, 0), (9, 63, 1), (130, 64, 0), (7, 100, 4), (64, 512, 0), (31, 513, 0), (3, 1000, 24), (17, 2048, 0), (9, 2049, 0),
              (40, 4100, 0), (5, 8192, 0), (600, 2500, 0), (2, 50001, 3), (1, 200003, 5), (1, 262144, 0), (520, 20000, 0)]
 
 
@@ -449,6 +544,8 @@ def test_token_logprobs_masks_and_ties(v, dt):
     t[11] = -100
     lp_check(x, t, top=min(v, 8))
     lp_check(x, t, top=0, ignore=int(t[6]))                # an ignored token inside the vocabulary
+    if 2048 < v < 10000:                                   # enough rows for a wave each
+        lp_check(x.repeat(150, 1), t.repeat(150), top=5)
 
 
 @pytest.mark.parametrize("dt", [BF16, F32])
@@ -598,6 +695,17 @@ def test_adamw_extreme_gradients(bits):
         assert torch.isfinite(opt.flat_p).all()
 
 
+@pytest.mark.parametrize("bits,n", [(32, 10_000_003), (8, 17_000_001)])
+def test_adamw_beyond_the_cache(bits, n):
+    """Buffers over 256 MiB: four blocks a wave, streaming accesses; the last wave's blocks are not all there."""
+    opt, g = make_opt(bits, shapes=[(n,), (77, 3)])
+    for _ in range(2):
+        opt.zero_grad()
+        for p in opt.params:
+            p.grad.add_(torch.randn(p.shape, device="cuda", generator=g) * 1e-3)
+        adamw_step_check(opt)
+
+
 def test_adamw_8bit_nonfinite_gradients_stay_with_their_elements():
     opt, g = make_opt(8, shapes=[(300,)])
     other, _ = make_opt(8, shapes=[(300,)])
@@ -668,6 +776,21 @@ def test_adamw_32bit_matches_torch():
         ta.step()
     for p, r in zip(opt.params, ref):
         assert float((p - r).abs().max()) <= 3 * 16 * U * (float(r.abs().max()) + 1)
+
+
+def test_adamw_buckets_and_frozen_parameters():
+    """The data-parallel buckets are slices of the flat gradient buffer, whose tensors begin at multiples of 256 here; a
+    parameter that needs no gradient is left alone."""
+    from vae_gan_amd.optim import FlatAdamW
+    from vae_gan_amd.train import DataParallel
+    ps = [torch.nn.Parameter(torch.ones(300, device="cuda")), torch.nn.Parameter(torch.ones(5, device="cuda"), requires_grad=False),
+          torch.nn.Parameter(torch.ones(256, device="cuda")), torch.nn.Parameter(torch.ones(2, 2, device="cuda"))]
+    opt = FlatAdamW(ps, lr=0.1, weight_decay=0.5)
+    assert opt.offsets == [0, 512, 768] and opt.numel == 1024 and opt._decay is None
+    assert DataParallel.span(opt, [ps[2]]) == (512, 768) and DataParallel.span(opt, [ps[2], ps[3]]) == (512, 1024)
+    opt.zero_grad()
+    opt.step()
+    assert torch.equal(ps[1], torch.ones(5, device="cuda")) and float((ps[0] - 0.95).abs().max()) <= 2 * U
 
 
 def test_training_step_with_adamw_and_checkpoint(tmp_path):

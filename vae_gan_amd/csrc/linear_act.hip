@@ -183,14 +183,15 @@ template <int N> __device__ __forceinline__ void la_wait_barrier() {
 }
 typedef __attribute__((address_space(3))) bf16x4* la_tr_t;
 
-// One operand's tile: R rows (of C) x KB bytes of k (64 or 128), in 16-byte pieces, stored so that the fragment reads below
+// One operand's tile: R rows (of C) x 128 bytes of k, in 16-byte pieces, stored so that the fragment reads below
 // touch every LDS bank once.
-//   k contiguous:   [row][KB / 16 pieces], piece p of row r in slot p ^ (r >> 1 & 7) (KB 64: p ^ (r >> 2 & 3))
+//   k contiguous:   [row][8 pieces], piece p of row r in slot p ^ (r >> 1 & 7)
 //   row contiguous: [k][R elements]; the 32-byte (f32: 64-byte) column groups of k exchanged by the bits of k in which the
 //                   lanes of one read differ
-template <typename T, bool TR, int R, int NTH, int KB> struct LaTile {
+constexpr int KB = 128;                              // bytes of k in a tile
+template <typename T, bool TR, int R, int NTH> struct LaTile {
   static constexpr int EB = sizeof(T), PIECE = 16 / EB, KT = KB / EB, LOADS = R * (KB / 16) / NTH, BYTES = R * KB, RB = R * EB;
-  static __device__ __forceinline__ int turn(int r) { return KB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+  static __device__ __forceinline__ int turn(int r) { return (r >> 1) & 7; }
   static constexpr int FRAG_READS = TR ? (EB == 2 ? 2 : 4) : 1;
   unsigned voff[LOADS];
   int kof[LOADS];
@@ -243,12 +244,12 @@ __device__ __forceinline__ int la_xcd(int bid, int nblk) {      // blocks of one
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
 }
 
-// WM x WN waves, each MT x NT products of 16 x 16; a ring of S tiles of KB bytes of k; one barrier a tile
-template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S, int KB>
+// WM x WN waves, each MT x NT products of 16 x 16; a ring of S tiles of k; one barrier a tile
+template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmParams p) {
   constexpr int NTH = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
-  typedef LaTile<T, TA, BM, NTH, KB> TileA;
-  typedef LaTile<T, TB, BN, NTH, KB> TileB;
+  typedef LaTile<T, TA, BM, NTH> TileA;
+  typedef LaTile<T, TB, BN, NTH> TileB;
   constexpr int STAGE = TileA::BYTES + TileB::BYTES, LOADS = TileA::LOADS + TileB::LOADS, KT = TileA::KT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -319,16 +320,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
 #pragma unroll
   for (int i = 0; i < FRAGS; ++i) read(0, smem, 0, i);
   int cur = 0;
-  auto next = [&]() {
+  for (int kt = kt0; kt < kt1; ++kt) {
+    multiply(0, smem + cur * STAGE, 1, false);
     la_wait_barrier<(S - 2) * LOADS>();              // the next tile is in LDS, and everyone has read this one
     cur = cur + 1 == S ? 0 : cur + 1;
-    begin();                                         // tile kt + S takes its place
-  };
-  for (int kt = kt0; kt < kt1; kt += KB == 128 ? 1 : 2) {      // past the last tile: zeros
-    if constexpr (KB == 64) next();
-    multiply(0, smem + cur * STAGE, KB == 64 ? 0 : 1, KB == 64);
-    if constexpr (KB == 64) end();
-    next();
+    begin();                                         // tile kt + S takes its place; past the last one: zeros
     multiply(1, smem + cur * STAGE, 0, true);
     end();
   }
@@ -574,7 +570,7 @@ static LaPlan la_plan(int64_t m, int64_t n, int64_t k, int dtype) {
   struct Cost { int tile, res; double lat, step, fixed; };
   static const Cost bf16[3] = {{64, 3, 0.26, 0.20, 2.5}, {128, 2, 0.68, 0.55, 3.5}, {256, 1, 1.50, 1.65, 6.0}};
   static const Cost f32[2] = {{64, 3, 0.6, 0.53, 3.0}, {128, 2, 2.0, 2.0, 5.0}};
-  const int64_t kt = vg_ceil_div(k * vg_elt_size(dtype), 128);
+  const int64_t kt = vg_ceil_div(k * vg_elt_size(dtype), KB);
   LaPlan best = {64, 1, (int)kt, 1e30};
   for (int i = 0; i < (dtype == VG_BF16 ? 3 : 2); ++i) {
     const Cost& c = dtype == VG_BF16 ? bf16[i] : f32[i];
@@ -618,11 +614,19 @@ static char* la_pack(LaOperand* o[2], int dtype, char* ws, hipStream_t st) {
   return ws;
 }
 
-template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S, int KB> static int la_tile_launch(GemmParams p, hipStream_t st) {
-  p.ktiles *= 128 / KB;                              // the plan counts 128 bytes of k
+// what the calling thread's last product ran on (vg_last_linear_act_kernel)
+static thread_local struct { int rows, tile, ta, tb, splits, f32; } la_last;
+extern "C" const char* vg_last_linear_act_kernel(void) {
+  static thread_local char name[64];
+  if (la_last.rows) snprintf(name, sizeof(name), "rows<%s,%d>", la_last.f32 ? "f32" : "bf16", la_last.rows);
+  else snprintf(name, sizeof(name), "tile<%s,%d,%c%c>%s", la_last.f32 ? "f32" : "bf16", la_last.tile, la_last.ta ? 't' : 'n', la_last.tb ? 't' : 'n', la_last.splits > 1 ? "+join" : "");
+  return name;
+}
+
+template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S> static int la_tile_launch(GemmParams p, hipStream_t st) {
   constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
   const int ring = S * (BM + BN) * KB, out = WM * WN * 8 * MT * (16 * NT + 4) * 4, lds = ring > out ? ring : out;
-  void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S, KB>;
+  void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S>;
   VG_HIP(vg_lds_attr((const void*)kernel, lds));
   const int64_t blocks = vg_ceil_div(p.m, BM) * vg_ceil_div(p.n, BN) * p.splits;
   VG_REQUIRE(blocks < (1LL << 31), "linear_act: %d x %d outputs are too many for one launch", p.m, p.n);
@@ -636,11 +640,12 @@ template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int d
   p.ktiles = pl.ktiles;
   p.ldp = (int)la_pitch(p.n);
   p.part = pl.splits > 1 ? (float*)ws : nullptr;
+  la_last = {0, pl.tile, TA, TB, pl.splits, dtype == VG_F32};
   int rc;
-  if (pl.tile == 64) rc = la_tile_launch<T, TA, TB, 2, 2, 2, 2, 3, 128>(p, st);
-  else if (pl.tile == 128) rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2, 128>(p, st);
+  if (pl.tile == 64) rc = la_tile_launch<T, TA, TB, 2, 2, 2, 2, 3>(p, st);
+  else if (pl.tile == 128) rc = la_tile_launch<T, TA, TB, 2, 2, 4, 4, 2>(p, st);
   else {
-    if constexpr (sizeof(T) == 2) rc = la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2, 128>(p, st);
+    if constexpr (sizeof(T) == 2) rc = la_tile_launch<T, TA, TB, 2, 4, 8, 4, 2>(p, st);
     else rc = VG_ERR_UNSUPPORTED;                    // not planned for f32, whose matrix rate binds at any size
   }
   if (rc) return rc;
@@ -685,6 +690,7 @@ template <typename T, typename TW, int MB> static void la_rows_launch(const Gemm
   else hipLaunchKernelGGL((gemm_rows_kernel<T, TW, MB, false>), grid, dim3(512), 0, st, p);
 }
 template <typename T, typename TW> static int la_rows(const GemmParams& p, hipStream_t st) {
+  la_last = {p.m <= 16 ? 16 : p.m <= 32 ? 32 : 64, 0, 0, 0, 1, sizeof(T) == 4};
   const bool aligned = p.k % (16 / sizeof(T)) == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 && (p.lda * sizeof(T)) % 16 == 0 && (p.ldb * sizeof(TW)) % 16 == 0;
   if (p.m <= 16) la_rows_launch<T, TW, 1>(p, aligned, st);
   else if (p.m <= 32) la_rows_launch<T, TW, 2>(p, aligned, st);

@@ -131,6 +131,7 @@ SIGNATURES = {
     "vg_linear_act_dgrad": (_I, [_P, _P, _I, _P, _P, _L, _L, _L, _I, _P]),
     "vg_linear_act_wgrad_ws_bytes": (C.c_size_t, [_P, _P, _L, _L, _L, _L, _I]),
     "vg_linear_act_wgrad": (_I, [_P, _P, _L, _P, _I, _P, _L, _L, _L, _I, _P]),
+    "vg_last_linear_act_kernel": (C.c_char_p, []),
     "vg_token_logprobs_ws_bytes": (C.c_size_t, [_L, _I, _I]),
     "vg_token_logprobs_fwd": (_I, [_P, _L, _P, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P]),
     "vg_token_logprobs_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
