@@ -139,8 +139,8 @@ class FlatAdamW(FlatAdam):
         super().__init__(params, lr, betas, eps)
         self.decays = [decay_filter is None or bool(decay_filter(p)) for p in self.params]
         ends = self.offsets[1:] + [self.numel]
-        flags = [int(d) for d, lo, hi in zip(self.decays, self.offsets, ends) for _ in range((hi - lo) // self.ALIGN)]
-        self._decay = None if all(self.decays) else torch.tensor(flags, dtype=torch.uint8, device=self.flat_p.device)
+        blocks = torch.tensor([(hi - lo) // self.ALIGN for lo, hi in zip(self.offsets, ends)])
+        self._decay = None if all(self.decays) else torch.tensor(self.decays).to(torch.uint8).repeat_interleave(blocks).to(self.flat_p.device)
 
     def _alloc_state(self, n: int, dev):
         if self.state_bits == 32:
