@@ -519,6 +519,31 @@ def test_token_logprobs(rows, v, pad, dt):
 
 
 @pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("rows,v,team", [(600, 51200, 256), (2100, 2560, 64), (2, 70400, 256)])
+def test_token_logprobs_best_in_few_places(rows, v, team, dt):
+    """Rows whose best are all in the hands of a few threads (more than are listed), few ranked logits in masked rows at either
+    end, and rows of equal values but for a few."""
+    g = gen(v)
+    x = torch.randn(rows, v, device="cuda", generator=g)
+    stripe = (torch.arange(v, device="cuda") // (16 // torch.tensor([], dtype=dt).element_size())) % team
+    x[0] = x[0] + 5 * (stripe % 50 == 3)
+    if rows > 2:
+        x[1] = -math.inf
+        x[1, v - 3:] = 1.0
+        x[2] = -math.inf
+        x[2, :5] = -2.0
+        x[3] = 0.5
+        x[3, v // 2: v // 2 + 3] = 0.75
+        x[4] = torch.where(stripe % 50 == 3, x[4], torch.full_like(x[4], -math.inf))
+        x[5] = 0.5
+        x[5, : v - 2] = -1.0
+    x = x.to(dt)
+    t = torch.randint(0, v, (rows,), device="cuda", generator=g)
+    for top in (1, 8, 32):
+        lp_check(x, t, top=top)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
 @pytest.mark.parametrize("v", [6, 70, 700, 2050, 5003, 70001])
 def test_token_logprobs_masks_and_ties(v, dt):
     g = gen(v)

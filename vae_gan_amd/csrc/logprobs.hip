@@ -214,7 +214,8 @@ template <int TEAM> struct LpLists {                 // of one team, in LDS
   static constexpr int CAND = LP_CAND * TEAM / 256;
   unsigned long long cand[CAND], best[4], win[LP_MAX_TOP];
   float tmax[TEAM];
-  int count;
+  unsigned char who[TEAM];           // threads whose elements are looked through once more
+  int count, whos;
   float bound;
 };
 template <typename T> struct LpUnit { const T* x; int64_t row; int split, j0, j1, a0, nvec; };
@@ -226,10 +227,13 @@ __device__ void lp_best(const LpParams& p, const LpUnit<T>& u, LpLists<TEAM>& l,
   typedef T vt __attribute__((ext_vector_type(VEC)));
   const int tid = threadIdx.x % TEAM, lane = tid & 63, wave = tid >> 6, h = u.a0 - u.j0, t0 = u.a0 + u.nvec * VEC;
   l.tmax[tid] = mine;
-  if (tid == 0) l.count = 0;
+  if (tid == 0) l.count = l.whos = 0;
+  if (tid < LP_MAX_TOP) l.win[tid] = 0;
   team_sync<TEAM>();
   // The k-th largest of the threads' maxima bounds the k-th largest element from below: k different elements reach it.
-  // One wave finds it bit by bit, then everything at or above it is gathered.
+  // One wave finds it bit by bit, then everything at or above it is gathered: out of the elements of those threads alone whose
+  // maximum reaches it, dealt to the whole team, so that the second look costs one access a thread and not one more pass
+  // (560 x 51415 f32, top 8: 47 -> 26 us).
   if (wave == 0) {
     unsigned o[TEAM / 64], t = 0;
 #pragma unroll
@@ -245,25 +249,52 @@ __device__ void lp_best(const LpParams& p, const LpUnit<T>& u, LpLists<TEAM>& l,
   }
   team_sync<TEAM>();
   const float low = l.bound;
-  auto gather = [&](float v, unsigned j) {
-    if ((v == v ? v : -__builtin_inff()) >= low) {
-      const int at = atomicAdd(&l.count, 1);
-      if (at < l.CAND) l.cand[at] = rank_key(v, j);
-    }
-  };
-  for (int q = tid; q < u.nvec; q += TEAM) {
-    const vt w = *(const vt*)(u.x + u.a0 + (int64_t)q * VEC);
+  bool above = low == -__builtin_inff();             // only what is larger than the bound: its equals may be too many to list
+  int n;
+  for (;;) {
+    auto gather = [&](float v, unsigned j) {
+      if (above ? v > low : v >= low) {
+        const int at = atomicAdd(&l.count, 1);
+        if (at < l.CAND) l.cand[at] = rank_key(v, j);
+      }
+    };
+    if (above ? mine > low : mine >= low) l.who[atomicAdd(&l.whos, 1)] = (unsigned char)tid;
+    team_sync<TEAM>();
+    const int each = (u.nvec + TEAM - 1) / TEAM, items = l.whos * each;
+    for (int it = tid; it < items; it += TEAM) {
+      const int w = it / each, q = (it - w * each) * TEAM + l.who[w];
+      if (q >= u.nvec) continue;
+      const vt v = *(const vt*)(u.x + u.a0 + (int64_t)q * VEC);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) gather((float)w[e], (unsigned)(u.a0 + q * VEC + e));
+      for (int e = 0; e < VEC; ++e) gather((float)v[e], (unsigned)(u.a0 + q * VEC + e));
+    }
+    if (tid < h) gather(ldf(u.x + u.j0 + tid), (unsigned)(u.j0 + tid));
+    if (tid < u.j1 - t0) gather(ldf(u.x + t0 + tid), (unsigned)(t0 + tid));
+    team_sync<TEAM>();
+    n = l.count;
+    if (above || n <= l.CAND) break;
+    above = true;                                    // a row of many equal values
+    team_sync<TEAM>();
+    if (tid == 0) l.count = l.whos = 0;
+    team_sync<TEAM>();
   }
-  if (tid < h) gather(ldf(u.x + u.j0 + tid), (unsigned)(u.j0 + tid));
-  if (tid < u.j1 - t0) gather(ldf(u.x + t0 + tid), (unsigned)(t0 + tid));
-  team_sync<TEAM>();
-  const int n = l.count;
-  if (n >= p.top && n <= l.CAND) {
-    if (wave == 0) best_of(l.cand, n, p.top, lane, [&](int k, unsigned long long key) { l.win[k] = key; });
+  if (n <= l.CAND) {
+    if (wave == 0) {
+      // of the bound's equals (of -inf: all that is masked), the first ones fill the places that are left
+      for (int base = u.j0; n < p.top && base < u.j1; base += 64) {
+        const int j = base + lane;
+        const float v = j < u.j1 ? ldf(u.x + j) : 0.f;
+        const bool equal = j < u.j1 && (v == v ? v : -__builtin_inff()) == low;
+        const unsigned long long which = __ballot(equal);
+        const int at = n + __popcll(which & ((1ull << lane) - 1));
+        if (equal && at < p.top) l.cand[at] = rank_key(v, (unsigned)j);
+        n = min(n + __popcll(which), p.top);
+      }
+      team_sync<64>();
+      best_of(l.cand, n, p.top, lane, [&](int k, unsigned long long key) { l.win[k] = key; });
+    }
   } else {
-    // so many equal values (a constant row), or so few that can be ranked, that the list does not hold the answer: one scan a place
+    // a few threads hold more above the bound than the list does (values that repeat with the threads' stride): one scan a place
     unsigned long long last = ~0ull;
     for (int k = 0; k < p.top; ++k) {
       unsigned long long b = 0;
