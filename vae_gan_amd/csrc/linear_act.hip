@@ -111,17 +111,21 @@ template <typename T> __device__ __forceinline__ void la_finish1(const GemmParam
   if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j];
   if (p.c_f32) ((float*)p.c)[o] = x; else ((T*)p.c)[o] = (T)x;
 }
+// Residuals are asked for ahead of the stores of other rows: loads and stores come back in the order of their issue, so a load
+// behind a store waits for it (16384 x 1024 x 4096 bf16, GELU, slopes and a residual: 227 us, 197 so).
+template <typename T> using Res8 = T __attribute__((ext_vector_type(8)));
+template <typename T> __device__ __forceinline__ void la_ask8(const GemmParams& p, int i, int j, Res8<T>& t) {
+  if (p.res && p.vec && i < p.m && j + 8 <= p.n) t = *(const Res8<T>*)((const T*)p.res + (int64_t)i * p.ldres + j);
+}
 // without an activation
-template <typename T> __device__ __forceinline__ void la_plain8(const GemmParams& p, int i, int j, float* v, const float* bias) {
+template <typename T> __device__ __forceinline__ void la_plain8(const GemmParams& p, int i, int j, float* v, const float* bias, const Res8<T>& res) {
   const int64_t o = (int64_t)i * p.n + j;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
   if (p.vec && j + 8 <= p.n) {
     if (p.res) {
-      float t[8];
-      get8((const T*)p.res + (int64_t)i * p.ldres + j, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += t[e];
+      for (int e = 0; e < 8; ++e) v[e] += (float)res[e];
     }
     if (p.c_f32) put8((float*)p.c + o, v); else put8((T*)p.c + o, v);
   } else {
@@ -133,11 +137,11 @@ template <typename T> __device__ __forceinline__ void la_plain8(const GemmParams
       }
   }
 }
-template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v, const float* bias) {
+template <typename T> __device__ __forceinline__ void la_finish8(const GemmParams& p, int i, int j, float* v, const float* bias, const Res8<T>& res) {
   typedef typename SlopeT<T>::type S;
   const int64_t o = (int64_t)i * p.n + j;
   if (p.vec && j + 8 <= p.n) {
-    float t[8], s[8];
+    float s[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias[e];
     if (p.act != VG_ACT_NONE) {
@@ -145,9 +149,8 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
       if (p.slope) put8((S*)p.slope + o, s);
     }
     if (p.res) {
-      get8((const T*)p.res + (int64_t)i * p.ldres + j, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += t[e];
+      for (int e = 0; e < 8; ++e) v[e] += (float)res[e];
     }
     if (p.c_f32) put8((float*)p.c + o, v); else put8((T*)p.c + o, v);
   } else {
@@ -331,10 +334,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
   la_wait_barrier<0>();                              // the zeros asked for past the end have landed: LDS is free
 
   // acc[u][v][r] of a lane: row 16 u + lane % 16, column 16 v + 4 (lane / 16) + r.
-  if (p.part || p.act == VG_ACT_NONE) {
+  constexpr bool WIDE = sizeof(T) == 4 || NT == 2;   // the four lanes of a row read all that the wave has of it, or a line
+  if (p.part || (p.act == VG_ACT_NONE && (WIDE || !p.res))) {
     // Two neighbouring 16 x 16 blocks exchange rows of lanes, after which a lane has eight neighbouring columns: of the left
     // block in lanes 0-15 and 32-47, of the right one in the others.
     const int i1 = i0 + wm * MT * 16 + (lane & 15), j1 = j0 + wn * NT * 16 + ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;
+    Res8<T> res[NT / 2][MT];
+    if (WIDE && !p.part && p.res) {
+#pragma unroll
+      for (int v = 0; v < NT; v += 2)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) la_ask8<T>(p, i1 + u * 16, j1 + v * 16, res[v / 2][u]);
+    }
 #pragma unroll
     for (int v = 0; v < NT; v += 2) {
       const int j = j1 + v * 16;
@@ -352,20 +363,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
         const int i = i1 + u * 16;
         if (i < p.m && j < p.n) {
           if (p.part) put8(p.part + ((int64_t)split * p.m + i) * p.ldp + j, x);
-          else la_plain8<T>(p, i, j, x, bias);
+          else la_plain8<T>(p, i, j, x, bias, res[v / 2][u]);
         }
       }
     }
     return;
   }
-  // With an activation: through LDS (half of the wave's rows at a time) into a loop, since sixteen copies of the activations
-  // would not stay in the instruction cache.
+  // Through LDS (half of the wave's rows at a time) into a loop: with an activation, since sixteen copies of it would not stay in
+  // the instruction cache; bf16 residuals, since the eight lanes of a row read whole lines (16384 x 1024 x 4096 without an
+  // activation: 170 us by halves of lines, 149 so).
   constexpr int LDW = 16 * NT + 4, HALF = MT / 2;
   static_assert(64 % (2 * NT) == 0, "a lane keeps its columns");
   float* st = (float*)smem + wave * 16 * HALF * LDW;
   const int c = (lane % (2 * NT)) * 8, j = j0 + wn * NT * 16 + c;
+  constexpr int ITER = NT * HALF / 2, BATCH = ITER < 4 ? ITER : 4;      // accesses of a lane to a half; how many residuals wait
+  const int iw = i0 + wm * MT * 16;
   float bias[8];
   la_bias8<T>(p, j, bias);
+  Res8<T> res[BATCH], next[BATCH];
+  auto ask = [&](int q) {                            // the q-th access of a lane is to row (q * 64 + lane) / (2 NT) of the wave's
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) la_ask8<T>(p, iw + ((q + b) * 64 + lane) / (2 * NT), j, next[b]);
+  };
+  ask(0);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -375,14 +395,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(const GemmPa
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 4
-    for (int t = 0; t < NT * HALF / 2; ++t) {
-      const int r = (t * 64 + lane) / (2 * NT);
-      const int i = i0 + (wm * MT + h * HALF) * 16 + r;
-      float v[8];
-      *(f32x4*)v = *(const f32x4*)(st + r * LDW + c);
-      *(f32x4*)(v + 4) = *(const f32x4*)(st + r * LDW + c + 4);
-      if (i < p.m && j < p.n) la_finish8<T>(p, i, j, v, bias);
+#pragma unroll 1
+    for (int t0 = 0; t0 < ITER; t0 += BATCH) {
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) res[b] = next[b];
+      if (h * ITER + t0 + BATCH < 2 * ITER) ask(h * ITER + t0 + BATCH);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const int r = ((t0 + b) * 64 + lane) / (2 * NT), i = iw + h * HALF * 16 + r;
+        float v[8];
+        *(f32x4*)v = *(const f32x4*)(st + r * LDW + c);
+        *(f32x4*)(v + 4) = *(const f32x4*)(st + r * LDW + c + 4);
+        if (i < p.m && j < p.n) la_finish8<T>(p, i, j, v, bias, res[b]);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -462,6 +487,8 @@ template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(co
   if (q >= (int64_t)p.m * per) return;
   const int i = (int)(q / per), j = (int)(q % per) * 8;
   float v[8], t[8];
+  Res8<T> res;
+  la_ask8<T>(p, i, j, res);
   get8(p.part + (int64_t)i * p.ldp + j, v);
   for (int s = 1; s < p.splits; ++s) {
     get8(p.part + ((int64_t)s * p.m + i) * p.ldp + j, t);
@@ -470,7 +497,7 @@ template <typename T> __global__ __launch_bounds__(256) void gemm_join_kernel(co
   }
   float bias[8];
   la_bias8<T>(p, j, bias);
-  la_finish8<T>(p, i, j, v, bias);
+  la_finish8<T>(p, i, j, v, bias, res);
 }
 
 // Matrices [rows][cols] (row stride ld) into [rows][pitch], the padding zeroed: both operands of a product in one launch, the
