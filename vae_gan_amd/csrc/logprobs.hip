@@ -155,10 +155,11 @@ template <typename T> __device__ __forceinline__ float token_logit(const LpParam
 }
 
 // ---- rows that fit a wave's registers ------------------------------------------------------------------------------------
-// lane l holds VEC-element accesses l, l + 64, ...
-template <typename T, int VEC, int NV>
+// lane l holds 16-byte accesses l, l + 64, ..., aligned to an element only (the machine's global memory instructions take that)
+template <typename T, int NV>
 __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
-  typedef T vt __attribute__((ext_vector_type(VEC)));
+  constexpr int VEC = Elt<T>::PIECE;
+  typedef T vt __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   const int lane = threadIdx.x & 63;
   const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
   if (row >= p.rows) return;
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = (i * 64 + lane) * VEC;
-    if (VEC > 1 && j + VEC <= p.vocab) {
+    if (j + VEC <= p.vocab) {
       const vt q = *(const vt*)(x + j);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[i * VEC + e] = (float)q[e];
@@ -439,6 +440,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tpr) {      // tpr: threads of a row (64 or 256)
   constexpr int VEC = Elt<T>::PIECE;
   typedef T vt __attribute__((ext_vector_type(VEC)));
+  typedef T ut __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));      // the gradient's rows may be aligned otherwise
   const int per = 256 / tpr, gl = threadIdx.x % tpr;
   const int64_t unit = blockIdx.x * (int64_t)per + threadIdx.x / tpr;
   const int64_t row = unit / p.splits;
@@ -459,17 +461,13 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tp
   };
   int hd = (int)(((16 - (uintptr_t)(x + j0) % 16) % 16) / sizeof(T));
   if (hd > j1 - j0) hd = j1 - j0;
-  if ((uintptr_t)(dx + j0 + hd) % 16) {              // the two rows are not aligned alike
-    for (int j = j0 + gl; j < j1; j += tpr) dx[j] = (T)grad(ldf(x + j), j);
-    return;
-  }
   const int a0 = j0 + hd, nvec = (j1 - a0) / VEC, t0 = a0 + nvec * VEC;
   for (int i = gl; i < nvec; i += tpr) {
     const vt q = *(const vt*)(x + a0 + (int64_t)i * VEC);
-    vt o;
+    ut o;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] = (T)grad((float)q[e], a0 + i * VEC + e);
-    *(vt*)(dx + a0 + (int64_t)i * VEC) = o;
+    *(ut*)(dx + a0 + (int64_t)i * VEC) = o;
   }
   if (gl < hd) dx[j0 + gl] = (T)grad(ldf(x + j0 + gl), j0 + gl);
   if (gl < j1 - t0) dx[t0 + gl] = (T)grad(ldf(x + t0 + gl), t0 + gl);
@@ -506,15 +504,11 @@ extern "C" size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top) {
 static const int64_t LP_WAVE_UNITS = 2048;          // two waves a SIMD
 template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
   if (lp_regs(p.vocab)) {
-    constexpr int V = Elt<T>::PIECE;
     const dim3 grid((unsigned)vg_ceil_div(p.rows, 4));
-    const bool vec = (uintptr_t)p.x % 16 == 0 && (p.ldx * sizeof(T)) % 16 == 0;
-#define LP_CASE(VEC, NV) \
-  if (p.vocab <= 64 * VEC * NV) { hipLaunchKernelGGL((lp_wave_kernel<T, VEC, NV>), grid, dim3(256), 0, st, p); return; }
-    if (vec) {
-      if constexpr (V == 4) { LP_CASE(4, 1) LP_CASE(4, 2) LP_CASE(4, 4) LP_CASE(4, 8) }
-      else { LP_CASE(8, 1) LP_CASE(8, 2) LP_CASE(8, 4) }
-    } else { LP_CASE(1, 4) LP_CASE(1, 8) LP_CASE(1, 16) LP_CASE(1, 32) }
+#define LP_CASE(NV) \
+  if (p.vocab <= 64 * Elt<T>::PIECE * NV) { hipLaunchKernelGGL((lp_wave_kernel<T, NV>), grid, dim3(256), 0, st, p); return; }
+    LP_CASE(1) LP_CASE(2) LP_CASE(4)
+    if constexpr (sizeof(T) == 4) { LP_CASE(8) }
 #undef LP_CASE
     return;
   }
