@@ -259,15 +259,22 @@ __device__ void lp_best(const LpParams& p, const LpUnit<T>& u, LpLists<TEAM>& l,
         if (at < l.CAND) l.cand[at] = rank_key(v, j);
       }
     };
-    if (above ? mine > low : mine >= low) l.who[atomicAdd(&l.whos, 1)] = (unsigned char)tid;
-    team_sync<TEAM>();
-    const int each = (u.nvec + TEAM - 1) / TEAM, items = l.whos * each;
-    for (int it = tid; it < items; it += TEAM) {
-      const int w = it / each, q = (it - w * each) * TEAM + l.who[w];
-      if (q >= u.nvec) continue;
+    auto look = [&](int q) {
       const vt v = *(const vt*)(u.x + u.a0 + (int64_t)q * VEC);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) gather((float)v[e], (unsigned)(u.a0 + q * VEC + e));
+    };
+    const bool holds = above ? mine > low : mine >= low;
+    const int each = (u.nvec + TEAM - 1) / TEAM;     // accesses of a thread
+    if (each <= 2) {                                 // nothing to deal
+      for (int q = holds ? tid : u.nvec; q < u.nvec; q += TEAM) look(q);
+    } else {
+      if (holds) l.who[atomicAdd(&l.whos, 1)] = (unsigned char)tid;
+      team_sync<TEAM>();
+      for (int it = tid, items = l.whos * each; it < items; it += TEAM) {
+        const int w = it / each, q = (it - w * each) * TEAM + l.who[w];
+        if (q < u.nvec) look(q);
+      }
     }
     if (tid < h) gather(ldf(u.x + u.j0 + tid), (unsigned)(u.j0 + tid));
     if (tid < u.j1 - t0) gather(ldf(u.x + t0 + tid), (unsigned)(t0 + tid));
