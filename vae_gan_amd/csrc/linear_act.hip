@@ -5,6 +5,8 @@
 // All three products are C[i][j] = sum_k A(i, k) B(j, k), each operand either with k contiguous (x, W, dz in the first two)
 // or with i / j contiguous (W in dx = dz W, both in dW): a tile of the first kind is read from LDS with 16-byte reads, one of
 // the second with transposing reads, so nothing is transposed in memory.
+#include <type_traits>
+
 #include "common.h"
 #include "rows.h"
 
@@ -543,33 +545,38 @@ __global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, co
   const int j = (blockIdx.x * 32 + cg) * 8;
   const int r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < m ? r0 + rows_per : m;
   float s[8] = {};
-  if (j + 8 <= n) {
+  auto rows = [&](auto whole) {                      // the last columns of a row that is no multiple of 8: element by element
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll 4
     for (int r = r0 + ry; r < r1; r += 8) {
       const int64_t o = (int64_t)r * n + j;
       float g[8], t[8];
-      get8(dy + o, g);
+      if constexpr (WHOLE) get8(dy + o, g);
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = j + e < n ? (float)dy[o + e] : 0.f;
+      }
       if (slope) {
-        get8(slope + o, t);
+        if constexpr (WHOLE) get8(slope + o, t);
+        else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] = j + e < n ? (float)slope[o + e] : 0.f;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] *= t[e];
-        put8(dz + o, g);
+        if constexpr (WHOLE) put8(dz + o, g);
+        else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j + e < n) dz[o + e] = (T)g[e];
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] += g[e];
     }
-  } else if (j < n) {
-    for (int r = r0 + ry; r < r1; r += 8) {
-      const int64_t o = (int64_t)r * n + j;
-#pragma unroll
-      for (int e = 0; e < 7; ++e) {
-        if (j + e >= n) break;
-        float g = (float)dy[o + e];
-        if (slope) { g *= (float)slope[o + e]; dz[o + e] = (T)g; }
-        s[e] += g;
-      }
-    }
-  }
+  };
+  if (j + 8 <= n) rows(std::true_type{});
+  else if (j < n) rows(std::false_type{});
   if (!part) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) fold[ry][cg * 8 + e] = s[e];
@@ -769,10 +776,10 @@ extern "C" int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int 
   return la_gemm(p, a, false, b, false, dtype, ws, (hipStream_t)stream);
 }
 
-// chunks of rows: enough blocks to fill the chip, at least 32 rows each so that the partial sums stay a small part of the traffic
+// chunks of rows: enough blocks to fill the chip, at least 16 rows each so that the partial sums stay a small part of the traffic
 static int la_dz_parts(int64_t m, int64_t n) {
   int64_t parts = vg_ceil_div(2048, vg_ceil_div(n, 256));
-  if (parts > vg_ceil_div(m, 32)) parts = vg_ceil_div(m, 32);
+  if (parts > vg_ceil_div(m, 16)) parts = vg_ceil_div(m, 16);
   return (int)parts;
 }
 extern "C" size_t vg_linear_act_dz_ws_bytes(int64_t m, int64_t n) {

@@ -156,18 +156,40 @@ template <typename T> __device__ __forceinline__ float token_logit(const LpParam
 
 // ---- rows that fit a wave's registers ------------------------------------------------------------------------------------
 // lane l holds 16-byte accesses l, l + 64, ..., aligned to an element only (the machine's global memory instructions take that)
-template <typename T, int NV>
+// GL lanes share a row (short rows: several to a wave; 65536 x 128 bf16: 18 us with a wave each, 6 with 16 lanes)
+template <int GL, typename V, typename F> __device__ __forceinline__ V group_fold(V v, F f) {
+#pragma unroll
+  for (int o = GL / 2; o > 0; o >>= 1) v = f(v, (V)__shfl_xor(v, o, 64));
+  return v;
+}
+template <int GL> __device__ __forceinline__ float group_max(float v) {
+  if constexpr (GL == 64) return wave_max64(v);
+  else return group_fold<GL>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int GL> __device__ __forceinline__ float group_sum(float v) {
+  if constexpr (GL == 64) return wave_sum64(v);
+  else return group_fold<GL>(v, [](float a, float b) { return a + b; });
+}
+template <int GL> __device__ __forceinline__ unsigned long long group_max_key(unsigned long long k) {
+  if constexpr (GL == 64) return wave_max_key(k);
+  else {
+    auto larger = [](unsigned a, unsigned b) { return a > b ? a : b; };
+    const unsigned hi = group_fold<GL>((unsigned)(k >> 32), larger);
+    return ((unsigned long long)hi << 32) | group_fold<GL>((unsigned)(k >> 32) == hi ? (unsigned)k : 0u, larger);
+  }
+}
+template <typename T, int GL, int NV>
 __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
   constexpr int VEC = Elt<T>::PIECE;
   typedef T vt __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
-  const int lane = threadIdx.x & 63;
-  const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x % GL;
+  const int64_t row = blockIdx.x * (int64_t)(256 / GL) + threadIdx.x / GL;
   if (row >= p.rows) return;
   const T* x = (const T*)p.x + row * p.ldx;
   float v[NV * VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int j = (i * 64 + lane) * VEC;
+    const int j = (i * GL + lane) * VEC;
     if (j + VEC <= p.vocab) {
       const vt q = *(const vt*)(x + j);
 #pragma unroll
@@ -180,10 +202,10 @@ __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
   float mx = v[0];
 #pragma unroll
   for (int i = 1; i < NV * VEC; ++i) mx = fmaxf(mx, v[i]);
-  Soft a = {wave_max64(mx), 0.f, 0.f};
+  Soft a = {group_max<GL>(mx), 0.f, 0.f};
   soft_add<NV * VEC>(a, v);
-  a.s = wave_sum64(a.s);
-  a.u = wave_sum64(a.u);
+  a.s = group_sum<GL>(a.s);
+  a.u = group_sum<GL>(a.u);
   if (lane == 0) finish_row(p, row, a, token_logit<T>(p, row));
   unsigned long long last = ~0ull;
   for (int k = 0; k < p.top; ++k) {
@@ -192,11 +214,11 @@ __global__ __launch_bounds__(256) void lp_wave_kernel(const LpParams p) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int j = (i * 64 + lane) * VEC + e;
+        const int j = (i * GL + lane) * VEC + e;
         const unsigned long long key = rank_key(v[i * VEC + e], (unsigned)j);
         if (j < p.vocab && key < last && key > best) best = key;
       }
-    last = wave_max_key(best);
+    last = group_max_key<GL>(best);
     if (lane == 0) put_top(p, row, k, last, a);
   }
 }
@@ -444,7 +466,7 @@ struct LpBwdParams {
   int vocab, splits, chunk;
 };
 template <typename T>
-__global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tpr) {      // tpr: threads of a row (64 or 256)
+__global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tpr) {      // tpr: threads of a row (8 .. 64 or 256)
   constexpr int VEC = Elt<T>::PIECE;
   typedef T vt __attribute__((ext_vector_type(VEC)));
   typedef T ut __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));      // the gradient's rows may be aligned otherwise
@@ -511,11 +533,13 @@ extern "C" size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top) {
 static const int64_t LP_WAVE_UNITS = 2048;          // two waves a SIMD
 template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
   if (lp_regs(p.vocab)) {
-    const dim3 grid((unsigned)vg_ceil_div(p.rows, 4));
-#define LP_CASE(NV) \
-  if (p.vocab <= 64 * Elt<T>::PIECE * NV) { hipLaunchKernelGGL((lp_wave_kernel<T, NV>), grid, dim3(256), 0, st, p); return; }
-    LP_CASE(1) LP_CASE(2) LP_CASE(4)
-    if constexpr (sizeof(T) == 4) { LP_CASE(8) }
+#define LP_CASE(GL, NV)                                                                                                                       \
+  if (p.vocab <= GL * Elt<T>::PIECE * NV) {                                                                                                   \
+    hipLaunchKernelGGL((lp_wave_kernel<T, GL, NV>), dim3((unsigned)vg_ceil_div(p.rows, 256 / GL)), dim3(256), 0, st, p);                      \
+    return;                                                                                                                                   \
+  }
+    LP_CASE(8, 1) LP_CASE(16, 1) LP_CASE(32, 1) LP_CASE(64, 1) LP_CASE(64, 2) LP_CASE(64, 4)
+    if constexpr (sizeof(T) == 4) { LP_CASE(64, 8) }
 #undef LP_CASE
     return;
   }
@@ -555,9 +579,11 @@ extern "C" int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int6
   if (rows == 0) return VG_OK;
   VG_REQUIRE(logits && tokens && lse && entropy && dx && lddx >= vocab, "token_logprobs_bwd: null pointer or a short row stride");
   LpBwdParams p = {logits, ldx, tokens, ignore, lse, entropy, dlogp, dent, dx, lddx, rows, vocab, 1, 0};
-  // a wave per row while the row is short; otherwise blocks, each with at most 32 KB of a row
-  const int tpr = vocab <= 4096 ? 64 : 256;
-  p.chunk = tpr == 64 ? (int)(vg_ceil_div(vocab, 8) * 8) : (1 << 14);
+  // up to a wave per row while the row is short (65536 x 128 bf16: 24 us with a wave, 9 with 16 lanes); otherwise blocks,
+  // each with at most 32 KB of a row
+  int tpr = vocab <= 4096 ? 64 : 256;
+  while (tpr > 8 && vocab <= tpr / 2 * (16 / vg_elt_size(dtype))) tpr /= 2;
+  p.chunk = tpr <= 64 ? (int)(vg_ceil_div(vocab, 8) * 8) : (1 << 14);
   p.splits = (int)vg_ceil_div(vocab, p.chunk);
   const int64_t units = rows * p.splits;
   const int64_t blocks = vg_ceil_div(units, 256 / tpr);
