@@ -544,6 +544,24 @@ def test_token_logprobs_best_in_few_places(rows, v, team, dt):
 
 
 @pytest.mark.parametrize("dt", [BF16, F32])
+def test_token_logprobs_equal_bests_far_from_the_front(dt):
+    """More equal bests than are listed, in the last part of a row, with none or a few better ones."""
+    g = gen(8)
+    x = torch.randn(520, 20011, device="cuda", generator=g).clamp_(-1, 1).to(dt)
+    x[0] = 0.0
+    x[0, 12345:] = 1.0
+    x[1] = x[0]
+    x[1, [20010, 7]] = 2.0
+    x[2, 10000:] = 30.0
+    x[3] = -math.inf
+    x[3, 19000:] = torch.finfo(dt).min
+    t = torch.randint(0, 20011, (520,), device="cuda", generator=g)
+    for top in (1, 5):
+        lp_check(x, t, top=top)
+        lp_check(x.repeat(4, 1), t.repeat(4), top=top)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
 @pytest.mark.parametrize("v", [6, 70, 700, 2050, 5003, 70001])
 def test_token_logprobs_masks_and_ties(v, dt):
     g = gen(v)
@@ -914,6 +932,68 @@ def test_a_training_step_of_a_code_model(dt, tol, bits):
 
 
 # ---------------------------------------------------------------------------------------------- streams and graphs
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_modules(dt):
+    """nn.LayerNorm on an NHWC activation with padded channels and nn.LinearAct on token rows with its input as the residual."""
+    from vae_gan_amd import lib as L
+    from vae_gan_amd import nn as vnn
+    g = gen(31)
+    norm, lin = vnn.LayerNorm(41).cuda(), vnn.LinearAct(48, 48, act=L.ACT_GELU).cuda()
+    x = torch.zeros(2, 5, 7, 48, device="cuda")
+    x[..., :41] = torch.randn(2, 5, 7, 41, device="cuda", generator=g)
+    x = x.to(dt)
+    y = norm(x)
+    ref = ln_oracle(x.reshape(-1, 48), norm.weight.detach(), norm.bias.detach(), None, 41, 1e-5, dt)
+    assert y.shape == x.shape and not y[..., 41:].any()
+    within(y.detach().reshape(-1, 48)[:, :41], *ref["y"], "y")
+    tokens = y.detach().reshape(70, 48).requires_grad_()
+    dy = torch.randn(70, 48, device="cuda", generator=g).to(dt)
+    once = torch.autograd.grad(lin(tokens, tokens), (tokens, lin.weight, lin.bias), dy, retain_graph=True)
+    other = tokens.detach().clone().requires_grad_()
+    apart = torch.autograd.grad(lin(tokens, other), (tokens, other, lin.weight, lin.bias), dy)
+    assert torch.equal(apart[1], dy) and torch.equal(once[1], apart[2]) and torch.equal(once[2], apart[3])
+    within(once[0].detach(), apart[0].double() + dy.double(), half(dt) * (apart[0].double() + dy.double()).abs(), "the input's two gradients")
+
+
+def test_second_derivatives_are_refused_and_a_graph_can_be_walked_twice():
+    from vae_gan_amd import ops
+    g = gen(32)
+    x = torch.randn(9, 40, device="cuda", generator=g, requires_grad=True)
+    w, b = torch.randn(40, 40, device="cuda", generator=g), torch.zeros(40, device="cuda")
+    t = torch.randint(0, 40, (9,), device="cuda", generator=g)
+    for f in (lambda: ops.layer_norm(x, b + 1, b), lambda: ops.linear_act(x, w, b, ACTS["silu"]), lambda: ops.token_logprobs(x, t)[0]):
+        out = f().sum()
+        first, = torch.autograd.grad(out, x, retain_graph=True)
+        assert torch.equal(first, torch.autograd.grad(out, x)[0])
+        with pytest.raises(RuntimeError, match="differentiated twice"):
+            torch.autograd.grad(f().sum(), x, create_graph=True)
+
+
+def test_two_streams_at_once():
+    """The same operators on two streams, each with its own workspaces, interleaved."""
+    from vae_gan_amd import ops
+    g = gen(33)
+    data = [[torch.randn(*s, device="cuda", generator=g).to(BF16) for s in ((700, 1030), (300, 1030), (300,))] for _ in range(2)]
+    t = torch.randint(0, 300, (700,), device="cuda", generator=g)
+
+    def run(x, w, b):
+        xg, wg = x.detach().requires_grad_(), w.detach().requires_grad_()
+        logp, ent, _, ta = ops.token_logprobs(ops.linear_act(xg, wg, b, ACTS["gelu"]), t, top=4)
+        return [logp.detach(), ta] + list(torch.autograd.grad(logp.sum() + ent.sum(), (xg, wg)))
+    want = [run(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in data]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(*data[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for out in got[i] for a, b in zip(out, want[i]))
+
+
 def test_operators_on_another_stream():
     from vae_gan_amd import ops
     x, w, b, res, dy = la_data(300, 256, 128, BF16, 3)

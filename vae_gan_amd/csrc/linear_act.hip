@@ -5,6 +5,8 @@
 // All three products are C[i][j] = sum_k A(i, k) B(j, k), each operand either with k contiguous (x, W, dz in the first two)
 // or with i / j contiguous (W in dx = dz W, both in dW): a tile of the first kind is read from LDS with 16-byte reads, one of
 // the second with transposing reads, so nothing is transposed in memory.
+// Bound by the matrix cores where the sizes fill the chip (bf16 16384 x 1024 x 4096: forward 131 us without an activation, dx 124,
+// dW 110 and 13 to join four parts: 1050, 1110 and 1120 TFLOP/s), by launches and latency below some 10 GFLOP.
 #include <type_traits>
 
 #include "common.h"

@@ -6,6 +6,8 @@
 // convention).  Bound by memory: x is read and y written once; backward reads x and dy and writes dx once.  A row is held
 // in the registers of GL lanes (a part of a wave, a wave, or the block's four waves) as NV accesses of VEC elements, so the
 // variance is that of the centred values (no cancellation of sum(x^2) - mu^2) at no second read.  All sums are f32.
+// 16384 x 512 bf16: forward 10 us (3.4 TB/s), backward 13 us (3.9 TB/s) and 3.5 us for the column sums; 65536 x 128 f32 forward
+// 13.5 us (5.0 TB/s), where the launch's own few us weigh less.
 #include "common.h"
 #include "rows.h"
 

@@ -122,7 +122,8 @@ class FlatAdamW(FlatAdam):
     gradient is not finite keeps NaN moments, as it would in 32 bits; the rest of its 256 is not touched.
 
     ``load_state_dict`` takes the hyperparameters of the file, as torch does: a ``FlatAdam`` file (32 bits) brings a weight
-    decay of 0.  8- and 32-bit states are not converted into each other (ValueError)."""
+    decay of 0.  8- and 32-bit states are not converted into each other (ValueError).  A step captured into a graph repeats its
+    learning rate and bias correction on every replay."""
 
     ALIGN = 256         # elements that share a scale (csrc/adamw.hip)
 
