@@ -543,6 +543,14 @@ def test_token_logprobs_best_in_few_places(rows, v, team, dt):
         lp_check(x, t, top=top)
 
 
+@pytest.mark.parametrize("rows,v,dt", [(2100, 10007, F32), (4200, 10007, BF16)])
+def test_token_logprobs_beyond_the_cache(rows, v, dt):
+    """Logits and gradient that take most of the last-level cache: the gradient leaves by other stores."""
+    x = (3 * torch.randn(rows, v, device="cuda", generator=gen(12))).to(dt)
+    t = torch.randint(0, v, (rows,), device="cuda", generator=gen(13))
+    lp_check(x, t, top=0)
+
+
 @pytest.mark.parametrize("dt", [BF16, F32])
 def test_token_logprobs_equal_bests_far_from_the_front(dt):
     """More equal bests than are listed, in the last part of a row, with none or a few better ones."""

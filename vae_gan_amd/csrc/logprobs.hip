@@ -2,8 +2,8 @@
 //   m = max x, s = sum e^(x-m), u = sum e^(x-m) (x-m):  logp = (x_t - m) - ln s,  H = ln s - u / s
 //   dx_j = dlogp ([j = t] - p_j) - dH p_j (ln p_j + H),  p_j = e^(x_j - lse)
 // Bound by memory: the forward reads the logits once, keeping (m, s, u) as running values that are rescaled when a larger
-// maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 70 and
-// 80 us, 805 MB at 5.3 TB/s).  Sums are f32; exponents are of x - m <= 0.
+// maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 71 and
+// 84 us, 805 MB at 5.2 TB/s, where the logits come from memory).  Sums are f32; exponents are of x - m <= 0.
 // Masked logits (-inf) count for nothing.  A row of nothing but -inf has no distribution: logp -inf, H 0, gradient 0.  A
 // NaN or +inf in a row makes its logp, H and gradient NaN.  tokens[r] == ignore: logp 0 and no gradient through logp; any
 // other token outside [0, vocab) gives logp NaN and no gradient through logp (it is never used as an index).
@@ -472,7 +472,11 @@ struct LpBwdParams {
   int64_t lddx, rows;
   int vocab, splits, chunk;
 };
-template <typename T>
+// STREAM (logits and gradient take more than LP_STREAM bytes, most of the last-level cache): stores that do not allocate there
+// leave it to the logits, and the copy of the gradient that follows does not wait for their eviction.  Forward, backward and a
+// read of the gradient, 16384 x 8192 bf16: 251 us so, 262 otherwise; 6000 x 8192: 94 and 100; 4096 x 8192, which fits: 70 and 66.
+#define LP_STREAM (160ll << 20)
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tpr) {      // tpr: threads of a row (8 .. 64 or 256)
   constexpr int VEC = Elt<T>::PIECE;
   typedef T vt __attribute__((ext_vector_type(VEC)));
@@ -503,7 +507,8 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdParams p, int tp
     ut o;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] = (T)grad((float)q[e], a0 + i * VEC + e);
-    *(ut*)(dx + a0 + (int64_t)i * VEC) = o;
+    if (STREAM) __builtin_nontemporal_store(o, (ut*)(dx + a0 + (int64_t)i * VEC));
+    else *(ut*)(dx + a0 + (int64_t)i * VEC) = o;
   }
   if (gl < hd) dx[j0 + gl] = (T)grad(ldf(x + j0 + gl), j0 + gl);
   if (gl < j1 - t0) dx[t0 + gl] = (T)grad(ldf(x + t0 + gl), t0 + gl);
@@ -595,8 +600,11 @@ extern "C" int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int6
   const int64_t units = rows * p.splits;
   const int64_t blocks = vg_ceil_div(units, 256 / tpr);
   VG_REQUIRE(blocks < (1LL << 31), "token_logprobs_bwd: %ld rows of %d logits are too many for one launch", (long)rows, vocab);
-  if (dtype == VG_BF16) hipLaunchKernelGGL(lp_bwd_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, tpr);
-  else hipLaunchKernelGGL(lp_bwd_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, tpr);
+  const bool stream_out = rows * (int64_t)vocab * 2 * vg_elt_size(dtype) > LP_STREAM;
+#define LP_BWD(T, S) hipLaunchKernelGGL((lp_bwd_kernel<T, S>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, tpr)
+  if (dtype == VG_BF16) { if (stream_out) LP_BWD(bf16_t, true); else LP_BWD(bf16_t, false); }
+  else { if (stream_out) LP_BWD(float, true); else LP_BWD(float, false); }
+#undef LP_BWD
   VG_LAUNCH_CHECK();
   return VG_OK;
 }
