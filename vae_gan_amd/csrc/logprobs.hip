@@ -16,24 +16,25 @@
 template <typename T> __device__ __forceinline__ float ldf(const T* p) { return (float)*p; }
 
 // A set of logits: m (its maximum), s = sum 2^d and u = sum 2^d d with d = x log2 e - c, c = m log2 e as rounded to f32: one
-// fused multiply-add and one exponential an element.  The rounding of c is the same in every d, so it cancels in d - log2 s.
-// Where x log2 e may leave the f32 range (rows at the type's lowest value), d = (x - m) log2 e.  Masked elements have d = -inf:
-// clamped where it multiplies, since 0 * -inf is NaN (2^-290 is 0 in f32).
+// fused multiply-add and one exponential an element.  The rounding of c is the same in every d, so it cancels in d - log2 s; it
+// grows with |m|, and 2^(it) has to fit the sums: from |m| = LP_FAR (2^20: 2^-4 there) up, d = (x - m) log2 e, whose rounding is
+// that of the distance alone.  Masked elements have d = -inf: clamped where it multiplies, since 0 * -inf is NaN (2^-290 is 0 in f32).
 #define LP_LOG2E 1.4426950408889634f
 #define LP_LN2 0.6931471805599453f
-#define LP_FAR 2e38f
+#define LP_FAR 0x1p20f
+#define LP_WIDE 2e38f      // x log2 e stays in range below it
 struct Soft { float m, s, u; };
 __device__ __forceinline__ float soft_base(float m) { return m == -__builtin_inff() ? 0.f : m; }
 __device__ __forceinline__ float soft_d(float x, float base) {
   return fabsf(base) < LP_FAR ? fmaf(x, LP_LOG2E, -(base * LP_LOG2E)) : (x - base) * LP_LOG2E;
 }
-// the same set about a larger maximum: the difference of the two c as they were rounded (not contracted), or the rounding
-// of the old one would stay in its sums
+// base log2 e - c, exactly: what every d about this base holds beside (x - base) log2 e
+__device__ __forceinline__ float soft_residual(float base) { return fabsf(base) < LP_FAR ? fmaf(base, LP_LOG2E, -(base * LP_LOG2E)) : 0.f; }
+// the same set about a larger maximum; the residual of the old base leaves its sums and that of the new one enters, or a set
+// that is joined from sets about near and far maxima would not be one sum
 __device__ __forceinline__ Soft soft_about(const Soft& a, float m) {
-#pragma clang fp contract(off)
   const float b = soft_base(m);
-  const bool near = fabsf(b) < LP_FAR && fabsf(a.m) < LP_FAR;
-  const float d = fmaxf(near ? a.m * LP_LOG2E - b * LP_LOG2E : (a.m - b) * LP_LOG2E, -290.f), e = __builtin_amdgcn_exp2f(d);
+  const float d = fmaxf((a.m - b) * LP_LOG2E + (soft_residual(b) - soft_residual(a.m)), -290.f), e = __builtin_amdgcn_exp2f(d);
   return Soft{m, a.s * e, e * (a.u + d * a.s)};
 }
 // (m, s, u) of two disjoint sets
@@ -44,18 +45,20 @@ __device__ __forceinline__ Soft soft_join(const Soft& a, const Soft& b) {
 }
 template <int N> __device__ __forceinline__ void soft_add(Soft& a, const float* x) {
   const float base = soft_base(a.m);
-  auto add = [&](float d) {
-    const float e = __builtin_amdgcn_exp2f(d);
+  const bool near = fabsf(base) < LP_FAR;
+  const float c = near ? base * LP_LOG2E : 0.f;
+  float y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = x[i];
+  if (!near) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] -= base;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = fmaf(y[i], LP_LOG2E, -c), e = __builtin_amdgcn_exp2f(d);
     a.s += e;
     a.u += e * fmaxf(d, -290.f);
-  };
-  if (fabsf(base) < LP_FAR) {
-    const float c = base * LP_LOG2E;
-#pragma unroll
-    for (int i = 0; i < N; ++i) add(fmaf(x[i], LP_LOG2E, -c));
-  } else {
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) add((x[i] - base) * LP_LOG2E);
   }
 }
 template <int N> __device__ __forceinline__ void soft_add_n(Soft& a, const float* x) {
@@ -136,7 +139,7 @@ struct LpParams {
 
 // ln p of a logit: (d - log2 s) ln 2, with d as it was summed; of one that is far down, whose d overflows, x - m - ln s
 __device__ __forceinline__ float soft_lnp(float x, const Soft& a) {
-  return fabsf(x) < LP_FAR ? (soft_d(x, a.m) - log2f(a.s)) * LP_LN2 : (x - a.m) - log2f(a.s) * LP_LN2;
+  return fabsf(x) < LP_WIDE ? (soft_d(x, a.m) - log2f(a.s)) * LP_LN2 : (x - a.m) - log2f(a.s) * LP_LN2;
 }
 __device__ __forceinline__ void finish_row(const LpParams& p, int64_t row, const Soft& a, float xt) {
   const bool empty = soft_empty(a);
