@@ -56,3 +56,17 @@ def test_token_logprobs_rows_and_parts_far_from_zero(repeat, v, dt):
         assert x.shape[0] >= 2048
     t = torch.randint(0, v, (x.shape[0],), device="cuda", generator=g)
     lp_check(x, t, top=min(v, 5))
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("v", [3, 2500, 70001])
+def test_token_logprobs_distances_near_the_end_of_the_range(v, dt):
+    """ln p = x - m - ln s is finite wherever x - m is, although (x - m) log2 e is not."""
+    x = torch.full((4, v), -math.inf, device="cuda")
+    x[0, :3] = torch.tensor([3e38, 0.0, 1e38])
+    x[1, :3] = torch.tensor([1.9e38, -1e38, 1.9e38])
+    x[2, :3] = torch.tensor([0.0, -3e38, -2.5e38])
+    x[3, :3] = torch.tensor([1.5e38, -1.5e38, 7.0])
+    x = x.to(dt)
+    lp_check(x, torch.ones(4, dtype=torch.int64, device="cuda"), top=3)
+    lp_check(x, torch.full((4,), 2, device="cuda"), top=3)

@@ -137,9 +137,11 @@ struct LpParams {
   unsigned long long* cand;           // [rows][splits][top]: its best
 };
 
-// ln p of a logit: (d - log2 s) ln 2, with d as it was summed; of one that is far down, whose d overflows, x - m - ln s
+// ln p of a logit: (d - log2 s) ln 2, with d as it was summed.  About a far maximum, and of a logit that is far down, d can
+// overflow where ln p does not: x - m - ln s (s about a far maximum has no residual; beside |x| >= LP_WIDE one does not count)
 __device__ __forceinline__ float soft_lnp(float x, const Soft& a) {
-  return fabsf(x) < LP_WIDE ? (soft_d(x, a.m) - log2f(a.s)) * LP_LN2 : (x - a.m) - log2f(a.s) * LP_LN2;
+  const float l2 = log2f(a.s);
+  return fabsf(a.m) < LP_FAR && fabsf(x) < LP_WIDE ? (soft_d(x, a.m) - l2) * LP_LN2 : (x - a.m) - l2 * LP_LN2;
 }
 __device__ __forceinline__ void finish_row(const LpParams& p, int64_t row, const Soft& a, float xt) {
   const bool empty = soft_empty(a);
