@@ -422,7 +422,8 @@ const char* vg_last_linear_act_kernel(void);
 
 /* Log probability of tokens[r] under row r of logits [rows][vocab] (row stride ldx), the row's entropy (nats) and its `top` best
  * alternatives (0..32; by value, then by lower place).  lse: [rows][2] f32 out for the backward pass (the row's maximum and log2 of its sum), or NULL.  -inf logits are
- * masked; a row of only -inf gives logp -inf, entropy 0, gradient 0; NaN or +inf in a row gives NaN (a NaN ranks as -inf among the
+ * masked: no probability and no gradient, except that a masked token in a row that allows others (logp -inf) gets dlogp at its place;
+ * a row of only -inf gives logp -inf, entropy 0, gradient 0; NaN or +inf in a row gives NaN (a NaN ranks as -inf among the
  * alternatives).  tokens[r] == ignore: logp 0 and no gradient through it; another token outside [0, vocab): logp NaN, no gradient
  * through it.  ws: vg_token_logprobs_ws_bytes (0: none needed). */
 size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top);

@@ -4,7 +4,8 @@
 // Bound by memory: the forward reads the logits once, keeping (m, s, u) as running values that are rescaled when a larger
 // maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 71 and
 // 84 us, 805 MB at 5.2 TB/s, where the logits come from memory).  Sums are f32; exponents are of x - m <= 0.
-// Masked logits (-inf) count for nothing.  A row of nothing but -inf has no distribution: logp -inf, H 0, gradient 0.  A
+// Masked logits (-inf) have p = 0, so by the formula no gradient, except a masked token in a row that allows others: logp -inf,
+// and dlogp at its place.  A row of nothing but -inf has no distribution: logp -inf, H 0, gradient 0.  A
 // NaN or +inf in a row makes its logp, H and gradient NaN.  tokens[r] == ignore: logp 0 and no gradient through logp; any
 // other token outside [0, vocab) gives logp NaN and no gradient through logp (it is never used as an index).
 #include "common.h"

@@ -1309,7 +1309,9 @@ def token_logprobs(logits, tokens, top: int = 0, ignore_index: int = -100):
     three f32, the last two None where ``top`` is 0.  Equal logits rank in the order of their places.  Gradients flow through
     ``logp`` and ``entropy``.
 
-    Logits of -inf are masked: no probability, no gradient.  A row of nothing else gives logp -inf, entropy 0 and gradient 0.
+    Logits of -inf are masked: no probability, and no gradient but one: where the token itself is masked in a row that allows
+    others, logp is -inf and its gradient goes to that logit unchanged (1 - p = 1), as through a logarithm of a softmax.  A row
+    of nothing else gives logp -inf, entropy 0 and gradient 0.
     NaN or +inf in a row gives NaN for it.  Positions whose token is ``ignore_index`` give logp 0 and take no gradient through
     it; any other token outside the vocabulary gives NaN (finding it here would need the host to wait for the GPU)."""
     out = L.native().token_logprobs(logits, tokens, top, ignore_index)
