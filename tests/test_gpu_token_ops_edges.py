@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_token_ops import lp_check
+from test_gpu_token_ops import lp_check, within
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -70,3 +70,45 @@ def test_token_logprobs_distances_near_the_end_of_the_range(v, dt):
     x = x.to(dt)
     lp_check(x, torch.ones(4, dtype=torch.int64, device="cuda"), top=3)
     lp_check(x, torch.full((4,), 2, device="cuda"), top=3)
+
+
+# ---------------------------------------------------------------------------------------------- layer norm far from zero
+# rows of a part of a wave, of a wave, of a block, and too long for its registers
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("c", [3, 41, 127, 1000, 1001, 5003, 8191, 9001])
+def test_layer_norm_of_constant_rows_is_the_bias(c, dt):
+    """A row of one value has the mean of that value, exactly, and no spread: xh = 0, whatever the width and the value."""
+    from vae_gan_amd import ops
+    g = gen(c)
+    x = torch.tensor([1000.0, 30000.0, 0.1, -1000.123, 3e-5, -7e8, 1 / 3, 0.0], device="cuda").to(dt)[:, None].repeat(1, c)
+    w, b = torch.randn(c, device="cuda", generator=g), torch.randn(c, device="cuda", generator=g)
+    dy = torch.randn(8, c, device="cuda", generator=g).to(dt)
+    xg, wg, bg = (t.detach().requires_grad_() for t in (x, w, b))
+    y = ops.layer_norm(xg, wg, bg)
+    assert torch.equal(y.detach(), b.to(dt).expand(8, c))
+    dx, dw, db = torch.autograd.grad(y, (xg, wg, bg), dy)
+    assert not dw.any()
+    gd = dy.double() * w.double()
+    r = 1e-5 ** -0.5
+    # the mean of c products and the difference: each term passes c / 256 + 64 roundings
+    tol = (64 + c / 256) * U * r * (gd.abs() + gd.abs().mean(1, keepdim=True))
+    within(dx, r * (gd - gd.mean(1, keepdim=True)), tol + torch.finfo(dt).eps / 2 * (r * (gd - gd.mean(1, keepdim=True))).abs(), "dx")
+
+
+@pytest.mark.parametrize("c", [41, 127, 1000, 5003, 9001])
+def test_layer_norm_of_a_small_spread_on_a_large_mean(c):
+    """x - mu is exact here (x and mu within a factor of 2), so xh is off by its own sums' roundings alone: n u of what they hold,
+    the spread and what the first mean was off by, n u |mu|; neither is of the size of u |mu| r."""
+    from vae_gan_amd import ops
+    g = gen(c)
+    x = 1000 + 0.01 * torch.randn(16, c, device="cuda", generator=g)
+    x[8:] = 30000 + torch.randn(8, c, device="cuda", generator=g)
+    w, b = torch.randn(c, device="cuda", generator=g), torch.randn(c, device="cuda", generator=g)
+    y = ops.layer_norm(x, w, b)
+    xd, n = x.double(), 64 + c / 256
+    var, mu = torch.var_mean(xd, 1, unbiased=False, keepdim=True)
+    r = (var + 1e-5).rsqrt()
+    xh = (xd - mu) * r
+    slack = (1 + n * U * mu.abs() * r).square()
+    ref = xh * w.double() + b.double()
+    within(y, ref, 2 * n * U * (xh.abs() + 1) * slack * w.double().abs() + 4 * U * (ref.abs() + b.double().abs()), "y")

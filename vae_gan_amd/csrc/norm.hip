@@ -5,7 +5,9 @@
 // Rows are [c valid + padding] elements with a row stride; padding columns of y / dx are written as zeros (the NHWC
 // convention).  Bound by memory: x is read and y written once; backward reads x and dy and writes dx once.  A row is held
 // in the registers of GL lanes (a part of a wave, a wave, or the block's four waves) as NV accesses of VEC elements, so the
-// variance is that of the centred values (no cancellation of sum(x^2) - mu^2) at no second read.  All sums are f32.
+// variance is that of the centred values (no cancellation of sum(x^2) - mu^2) at no second read.  All sums are f32; the mean of
+// the centred values, which is what the first mean's rounding left in them, is taken off them again: constant rows are exactly
+// centred and y = b, where a mean one step off would be raised by r, up to 316 at eps = 1e-5.
 // 16384 x 512 bf16: forward 10 us (3.4 TB/s), backward 13 us (3.9 TB/s) and 3.5 us for the column sums; 65536 x 128 f32 forward
 // 13.5 us (5.0 TB/s), where the launch's own few us weigh less.
 #include "common.h"
@@ -59,12 +61,16 @@ template <typename T, int VEC, bool PART> __device__ __forceinline__ void st_vec
 }
 
 // sum over the GL lanes that share a row; every lane gets it.  GL == 256: through LDS (red: one slot per wave and value)
-template <int GL> __device__ __forceinline__ float row_sum(float v, float* red, int slot) {
+template <int GL> __device__ __forceinline__ float lane_sum(float v) {
   if constexpr (GL >= 64) v = wave_sum64(v);
   else {
 #pragma unroll
     for (int o = GL / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   }
+  return v;
+}
+template <int GL> __device__ __forceinline__ float row_sum(float v, float* red, int slot) {
+  v = lane_sum<GL>(v);
   if constexpr (GL > 64) {
     if ((threadIdx.x & 63) == 0) red[slot * 4 + (threadIdx.x >> 6)] = v;
     __syncthreads();
@@ -72,15 +78,26 @@ template <int GL> __device__ __forceinline__ float row_sum(float v, float* red, 
   }
   return v;
 }
+// two sums with one barrier between them, in slots `slot` and `slot` + 1
+template <int GL> __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int slot) {
+  a = lane_sum<GL>(a);
+  b = lane_sum<GL>(b);
+  if constexpr (GL > 64) {
+    if ((threadIdx.x & 63) == 0) { red[slot * 4 + (threadIdx.x >> 6)] = a; red[slot * 4 + 4 + (threadIdx.x >> 6)] = b; }
+    __syncthreads();
+    a = (red[slot * 4] + red[slot * 4 + 1]) + (red[slot * 4 + 2] + red[slot * 4 + 3]);
+    b = (red[slot * 4 + 4] + red[slot * 4 + 5]) + (red[slot * 4 + 6] + red[slot * 4 + 7]);
+  }
+}
 
 template <typename T, int VEC, int GL, int NV, bool PART>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
                                                      const float* __restrict__ b, T* __restrict__ y, int64_t ldy,
                                                      float* __restrict__ stats, int64_t rows, int c, int cs, float eps) {
-  __shared__ float red[16];
+  __shared__ float red[24];
   constexpr int RPB = 256 / GL;
   const int gl = threadIdx.x % GL;
-  const float inv = 1.f / (float)c;
+  const float n = (float)c;
   float wv[NV][VEC], bv[NV][VEC];                    // zero in the padding: y comes out as 0 there
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -98,7 +115,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, in
   const int64_t step = (int64_t)gridDim.x * RPB;
   int turn = 0;
   fetch(blockIdx.x * (int64_t)RPB + threadIdx.x / GL);
-  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += step, turn ^= 2) {
+  for (int64_t r0 = blockIdx.x * (int64_t)RPB; r0 < rows; r0 += step, turn ^= 3) {
     const int64_t row = r0 + threadIdx.x / GL;
     const bool live = row < rows;                     // dead groups still take part in the shuffles and barriers
     float v[NV][VEC];
@@ -111,25 +128,28 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, in
         s += v[i][e];
       }
     fetch(row + step);
-    const float mu = row_sum<GL>(s, red, turn) * inv;
-    float q = 0.f;
+    const float mu = row_sum<GL>(s, red, turn) / n;
+    float q = 0.f, rest = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        v[i][e] -= mu;
-        q += (i * GL + gl) * VEC + e < c ? v[i][e] * v[i][e] : 0.f;
+        v[i][e] = (i * GL + gl) * VEC + e < c ? v[i][e] - mu : 0.f;
+        rest += v[i][e];
+        q += v[i][e] * v[i][e];
       }
-    const float r = 1.f / sqrtf(row_sum<GL>(q, red, turn + 1) * inv + eps);
+    row_sum2<GL>(rest, q, red, turn + 1);
+    rest /= n;
+    const float r = 1.f / sqrtf(fmaxf(q / n - rest * rest, 0.f) + eps);
     if (!live) continue;
-    if (stats && gl == 0) { stats[2 * row] = mu; stats[2 * row + 1] = r; }
+    if (stats && gl == 0) { stats[2 * row] = mu + rest; stats[2 * row + 1] = r; }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * GL + gl) * VEC;
       if (col >= cs) break;
       float o[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] = col + e < c ? v[i][e] * r * wv[i][e] + bv[i][e] : 0.f;
+      for (int e = 0; e < VEC; ++e) o[e] = col + e < c ? (v[i][e] - rest) * r * wv[i][e] + bv[i][e] : 0.f;
       st_vec<T, VEC, PART>(y + row * ldy + col, o, cs - col);
     }
   }
@@ -140,17 +160,19 @@ template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
                                                           const float* __restrict__ b, T* __restrict__ y, int64_t ldy,
                                                           float* __restrict__ stats, int c, int cs, float eps) {
-  __shared__ float red[8];
+  __shared__ float red[12];
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
   float s = 0.f;
   for (int i = threadIdx.x; i < c; i += 256) s += (float)xr[i];
   const float mu = row_sum<256>(s, red, 0) / (float)c;
-  float q = 0.f;
-  for (int i = threadIdx.x; i < c; i += 256) { const float d = (float)xr[i] - mu; q += d * d; }
-  const float r = 1.f / sqrtf(row_sum<256>(q, red, 1) / (float)c + eps);
-  if (stats && threadIdx.x == 0) { stats[2 * row] = mu; stats[2 * row + 1] = r; }
-  for (int i = threadIdx.x; i < cs; i += 256) y[row * ldy + i] = (T)(i < c ? ((float)xr[i] - mu) * r * w[i] + b[i] : 0.f);
+  float q = 0.f, rest = 0.f;
+  for (int i = threadIdx.x; i < c; i += 256) { const float d = (float)xr[i] - mu; rest += d; q += d * d; }
+  row_sum2<256>(rest, q, red, 1);
+  rest /= (float)c;
+  const float r = 1.f / sqrtf(fmaxf(q / (float)c - rest * rest, 0.f) + eps);
+  if (stats && threadIdx.x == 0) { stats[2 * row] = mu + rest; stats[2 * row + 1] = r; }
+  for (int i = threadIdx.x; i < cs; i += 256) y[row * ldy + i] = (T)(i < c ? ((float)xr[i] - mu - rest) * r * w[i] + b[i] : 0.f);
 }
 
 // dx of the rows of this block (block-strided), and the block's partial sums of dw and db: part[block][2][c]
