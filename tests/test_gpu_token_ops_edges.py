@@ -112,3 +112,43 @@ def test_layer_norm_of_a_small_spread_on_a_large_mean(c):
     slack = (1 + n * U * mu.abs() * r).square()
     ref = xh * w.double() + b.double()
     within(y, ref, 2 * n * U * (xh.abs() + 1) * slack * w.double().abs() + 4 * U * (ref.abs() + b.double().abs()), "y")
+
+
+# ---------------------------------------------------------------------------------------------- activations at their ends
+def act_values(z, act, dt, rows):
+    """act(z) and the gradient of its sum, for values z, through a product that is exact (one input, weight 1): few rows, or tiles
+    whose other columns repeat the values."""
+    from vae_gan_amd import ops
+    n = 1 if rows else 64
+    x = z.reshape(-1, 1).to(dt).requires_grad_()
+    w = torch.ones(n, 1, dtype=dt, device="cuda")
+    parts = x.split(60) if rows else (x,)
+    y = torch.cat([ops.linear_act(p, w, None, act) for p in parts])
+    assert all(torch.equal(y[:, 0], y[:, j]) for j in range(n))
+    dy = torch.zeros_like(y)
+    dy[:, 0] = 1
+    (dx,) = torch.autograd.grad(y, x, dy)
+    return y.detach()[:, 0], dx[:, 0]
+
+
+@pytest.mark.parametrize("rows", [True, False])
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_gelu_keeps_its_negative_tail(dt, rows):
+    """z Phi(z) and Phi(z) + z phi(z) relative to the size of their terms.  Phi(-|z|) is off by 4.1e-6 (bf16; measured against erfc
+    over a grid in f32 arithmetic) or 9 u (f32) and an ulp of the reciprocal; e^(-z^2/2) by 2 u and, beside bf16, by the rounding
+    of z^2/2 log2 e: z^2 u.  f32 results below 2^-126 have no full mantissa: an absolute 2^-126 for them."""
+    from vae_gan_amd import lib as L
+    z = torch.cat([torch.linspace(-12.5, 9, 700, device="cuda"), torch.tensor([0.0, -0.0, 1e-6, -1e-6, 40.0, 1e20], device="cuda")]).to(dt)
+    y, dx = act_values(z, L.ACT_GELU, dt, rows)
+    zd = z.double()
+    phi, pdf = torch.special.erfc(-zd / math.sqrt(2)) / 2, (-zd * zd / 2).exp() / math.sqrt(2 * math.pi)
+    own = 4.1e-6 + 8 * U if dt == BF16 else 16 * U
+    rel = own + (4 + (zd * zd if dt == BF16 else 0 * zd)) * U
+    h = torch.finfo(dt).eps / 2
+    within(y, zd * phi, (zd * phi).abs() * (h + rel.clamp_max(1)) + 2.0 ** -126, "y")
+    slope, mag = phi + zd * pdf, phi + (zd * pdf).abs()
+    if dt == BF16:       # kept in f16 (half a step 2^-11, 2^-25 for its subnormals), rounded to bf16 as dz
+        tol = slope.abs() * (2.0 ** -11 + 2.0 ** -8) * 1.001 + 2.0 ** -25
+    else:
+        tol = slope.abs() * h + 2.0 ** -126
+    within(dx, slope, tol + mag * rel.clamp_max(1), "slope")

@@ -15,10 +15,27 @@
 typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef _Float16 f16_t;
 
-// act(z) and act'(z), sharing the exponential.  Phi(-|z|) of GELU is half of Abramowitz & Stegun 7.1.26 (erfc to 1.5e-7, from
-// the same e^(-z^2/2) as the density): a library erf costs four times the instructions, and 67 M of them took as long as the
+// Phi(-|x|) = e^(-x^2/2) t P(t) with t = 1 / (1 + p |x|), and that exponential, which the density needs too.  P is fitted to the
+// smallest relative error over |x| <= 13.5 (e^(-x^2/2) is 0 in f32 from there on), so z Phi(z) keeps its leading digits in the
+// negative tail: 3.7e-6 of Phi with six coefficients, for results in bf16 (2^-9), 6.1e-8 with eight, for f32, where x^2 is
+// carried in two parts as well.  A library erfc costs four times the instructions, and 67 M of them took as long as the
 // product of 16384 x 1024 x 4096 itself.
-template <int N> __device__ __forceinline__ void la_act(float* z, int act, float* s) {
+template <typename T> __device__ __forceinline__ float la_phi(float x, float& e) {
+  const float a = fabsf(x), h = x * x;
+  if constexpr (sizeof(T) == 2) {
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.307628282f * a);
+    e = __expf(-0.5f * h);
+    return e * t * (0.122990536f + t * (0.118537826f + t * (0.137324485f + t * (0.00529493169f + t * (0.191671309f + t * -0.0758208932f)))));
+  } else {
+    const float t = 1.f / (1.f + 0.305121229f * a), low = h < __builtin_inff() ? fmaf(x, x, -h) : 0.f;
+    e = expf(-0.5f * h);
+    e -= e * 0.5f * low;
+    return e * t * (0.121686477f + t * (0.122538544f + t * (0.103320019f + t * (0.121442011f + t * (-0.0387208932f +
+           t * (0.186413127f + t * (-0.153564337f + t * 0.0368851234f)))))));
+  }
+}
+// act(z) and act'(z), sharing the exponential
+template <typename T, int N> __device__ __forceinline__ void la_act(float* z, int act, float* s) {
   switch (act) {                                     // one branch for all N: their exponentials overlap
     case VG_ACT_LRELU:
 #pragma unroll
@@ -31,9 +48,9 @@ template <int N> __device__ __forceinline__ void la_act(float* z, int act, float
     case VG_ACT_GELU:
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float x = z[i], e = __expf(-0.5f * x * x), t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * fabsf(x));
-        const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-        const float phi = x < 0.f ? q : 1.f - q;
+        const float x = z[i];
+        float e;
+        const float q = la_phi<T>(x, e), phi = x < 0.f ? q : 1.f - q;
         z[i] = x * phi;
         s[i] = phi + x * e * 0.39894228040143268f;
       }
@@ -119,7 +136,7 @@ template <typename T> __device__ __forceinline__ void la_finish1(const GemmParam
   const int64_t o = (int64_t)i * p.n + j;
   float s = 1.f;
   x += bias;
-  la_act<1>(&x, p.act, &s);
+  la_act<T, 1>(&x, p.act, &s);
   if (p.slope) ((S*)p.slope)[o] = (S)s;
   if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j];
   if (p.c_f32) ((float*)p.c)[o] = x; else ((T*)p.c)[o] = (T)x;
@@ -159,7 +176,7 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias[e];
     if (p.act != VG_ACT_NONE) {
-      la_act<8>(v, p.act, s);
+      la_act<T, 8>(v, p.act, s);
       if (p.slope) put8((S*)p.slope + o, s);
     }
     if (p.res) {
