@@ -152,3 +152,25 @@ def test_gelu_keeps_its_negative_tail(dt, rows):
     else:
         tol = slope.abs() * h + 2.0 ** -126
     within(dx, slope, tol + mag * rel.clamp_max(1), "slope")
+
+
+@pytest.mark.parametrize("rows", [True, False])
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_logistic_activations_keep_both_tails(act, dt, rows):
+    """Relative to the size of their terms: e^-|z| is off by 2 u (f32), or by 2 u + 2 |z| u (bf16: two roundings of |z| log2 e); the
+    quotient and the products by at most 6 u more.  In f32 a slope is kept to where it ends (2^-126)."""
+    from vae_gan_amd import lib as L
+    z = torch.cat([torch.linspace(-80, 80, 700, device="cuda"), torch.linspace(-9, 9, 300, device="cuda"), torch.tensor([0.0, -0.0, 1e-6], device="cuda")]).to(dt)
+    y, dx = act_values(z, L.ACT_SIGMOID if act == "sigmoid" else L.ACT_SILU, dt, rows)
+    zd = z.double()
+    p, q = 1 / (1 + (-zd).exp()), 1 / (1 + zd.exp())
+    h = torch.finfo(dt).eps / 2
+    rel = (8 + (2 * zd.abs() if dt == BF16 else 0 * zd)) * U
+    value, slope, mag = (p, p * q, p * q) if act == "sigmoid" else (zd * p, p * (1 + zd * q), p * (1 + zd.abs() * q))
+    within(y, value, value.abs() * (h + rel) + 2.0 ** -126, "y")
+    if dt == BF16:       # kept in f16 (half a step 2^-11, 2^-25 for its subnormals), rounded to bf16 as dz
+        tol = slope.abs() * (2.0 ** -11 + 2.0 ** -8) * 1.001 + 2.0 ** -25
+    else:
+        tol = slope.abs() * h + 2.0 ** -126
+    within(dx, slope, tol + mag * 2 * rel, "slope")

@@ -34,6 +34,14 @@ template <typename T> __device__ __forceinline__ float la_phi(float x, float& e)
            t * (0.186413127f + t * (-0.153564337f + t * 0.0368851234f)))))));
   }
 }
+// p = 1 / (1 + e^-x) and q = 1 - p, both from e^-|x| in (0, 1]: neither is a difference, so p's slope p q keeps its leading
+// digits on either side.  Results in f32 take the library's exponential and a division (the matrix cores bind there), results in
+// bf16 the machine's base-2 exponential (|x| 2^-24 of itself) and reciprocal.
+template <typename T> __device__ __forceinline__ void la_logistic(float x, float& p, float& q) {
+  const float e = sizeof(T) == 2 ? __expf(-fabsf(x)) : expf(-fabsf(x)), t = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+  p = x < 0.f ? e * t : t;
+  q = x < 0.f ? t : e * t;
+}
 // act(z) and act'(z), sharing the exponential
 template <typename T, int N> __device__ __forceinline__ void la_act(float* z, int act, float* s) {
   switch (act) {                                     // one branch for all N: their exponentials overlap
@@ -43,7 +51,12 @@ template <typename T, int N> __device__ __forceinline__ void la_act(float* z, in
       break;
     case VG_ACT_SIGMOID:
 #pragma unroll
-      for (int i = 0; i < N; ++i) { z[i] = __builtin_amdgcn_rcpf(1.f + __expf(-z[i])); s[i] = z[i] * (1.f - z[i]); }
+      for (int i = 0; i < N; ++i) {
+        float p, q;
+        la_logistic<T>(z[i], p, q);
+        z[i] = p;
+        s[i] = p * q;
+      }
       break;
     case VG_ACT_GELU:
 #pragma unroll
@@ -58,9 +71,11 @@ template <typename T, int N> __device__ __forceinline__ void la_act(float* z, in
     case VG_ACT_SILU:
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float x = z[i], p = __builtin_amdgcn_rcpf(1.f + __expf(-x));
+        const float x = z[i];
+        float p, q;
+        la_logistic<T>(x, p, q);
         z[i] = x * p;
-        s[i] = p * (1.f + x * (1.f - p));
+        s[i] = p * (1.f + x * q);
       }
       break;
     default: break;
