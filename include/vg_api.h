@@ -398,7 +398,7 @@ int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
 
 /* y = act(x W^T + bias) + res: x [m][k] (row stride ldx), w [n][k] in w_dtype (`dtype`, or VG_F32: rounded to `dtype` for the
  * products), y [m][n]; bias [n] in bias_dtype (`dtype` or VG_F32) or NULL; res [m][n] (row stride ldres) or NULL.  slope: NULL, or
- * [m][n] for act'(x W^T + bias), which the backward pass of an activation needs (2 bytes each (f16) for VG_BF16, f32 for VG_F32).
+ * [m][n] for act'(x W^T + bias), which vg_linear_act_dz takes (f16 of 2^14 times it for VG_BF16, f32 of itself for VG_F32).
  * f32 accumulation.  n, k < 2^20.  ws: the bytes that the _ws_bytes function names for the same operands (NULL for 0), aligned to 256. */
 size_t vg_linear_act_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype);
 int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int w_dtype, const void* bias, int bias_dtype, const void* res,

@@ -174,3 +174,21 @@ def test_logistic_activations_keep_both_tails(act, dt, rows):
     else:
         tol = slope.abs() * h + 2.0 ** -126
     within(dx, slope, tol + mag * 2 * rel, "slope")
+
+
+@pytest.mark.parametrize("rows", [True, False])
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+def test_small_slopes_beside_bf16(act, rows):
+    """A slope is kept as 2^14 times itself in f16: half a step of 2^-11 relative down to 2^-28, an absolute 2^-39 below; then one
+    rounding of dz to bf16.  (e^-|z| itself: 2 u + 2 |z| u.)"""
+    from vae_gan_amd import lib as L
+    z = torch.cat([torch.linspace(-27, -8, 400, device="cuda"), torch.linspace(8, 27, 400, device="cuda")]).to(BF16)
+    _, dx = act_values(z, {"sigmoid": L.ACT_SIGMOID, "silu": L.ACT_SILU, "gelu": L.ACT_GELU}[act], BF16, rows)
+    zd = z.double()
+    p, q = 1 / (1 + (-zd).exp()), 1 / (1 + zd.exp())
+    phi, pdf = torch.special.erfc(-zd / math.sqrt(2)) / 2, (-zd * zd / 2).exp() / math.sqrt(2 * math.pi)
+    slope, rel = {"sigmoid": (p * q, 2 * (8 + 2 * zd.abs()) * U), "silu": (p * (1 + zd * q), 3 * (8 + 2 * zd.abs()) * U),
+                  "gelu": (phi + zd * pdf, 5e-6 + (8 + zd * zd) * U)}[act]
+    within(dx, slope, slope.abs() * (2.0 ** -11 + 2.0 ** -8 + rel) * 1.001 + 2.0 ** -39, "slope")
+    if act == "sigmoid":
+        assert bool((dx[z > -26] > 0)[:100].all())

@@ -1,7 +1,11 @@
 // y = act(x W^T + b) + res and its gradient, x [M][K] and W [N][K] row-major, bf16 or f32, accumulated in f32 on the matrix
 // cores.  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  dres = dy.
-// The forward stores act'(z) beside y when a gradient will be wanted (in f16 for bf16 tensors: 2^-12 relative, where a z or a
-// slope rounded to bf16 would add an error as large as the gradient's own rounding).
+// The forward stores act'(z) beside y when a gradient will be wanted.  For bf16 tensors 2^14 act'(z) in f16: at most 2^-11
+// relative, where a z or a slope rounded to bf16 would add an error as large as the gradient's own rounding; the factor (slopes
+// are below 1.2, f16 ends at 65504) keeps that accuracy down to slopes of 2^-28, and anything above 2^-39 from becoming 0
+// (a sigmoid or SiLU at z = -26; beside bf16 gradients, whose own range is longer, smaller ones are lost).
+// dz is rounded to x's type before the two products of the backward pass, since bf16 matrix instructions take nothing wider:
+// dx and dW of 16384 x 1024 x 4096 are off by 2.4e-3 of their size where their own rounding alone gives 1.7e-3.
 // All three products are C[i][j] = sum_k A(i, k) B(j, k), each operand either with k contiguous (x, W, dz in the first two)
 // or with i / j contiguous (W in dx = dz W, both in dW): a tile of the first kind is read from LDS with 16-byte reads, one of
 // the second with transposing reads, so nothing is transposed in memory.
@@ -92,7 +96,7 @@ struct GemmParams {
   int bias_f32;
   const void* res;              // [m][n], row stride ldres, or null
   int64_t ldres;
-  void* slope;                  // [m][n] act'(z) out (f16 for bf16, f32 for f32), or null
+  void* slope;                  // [m][n] act'(z) out (f16, 2^14 times, for bf16; f32 for f32), or null
   int act;
   float* part;                  // split k: [splits][m][ldp] f32 partial sums instead of C
   int splits, ldp, ktiles;      // ktiles: of one split
@@ -112,8 +116,8 @@ template <> __device__ __forceinline__ f32x4 la_mma<float>(u32x4 a, u32x4 b, f32
 
 // ---- epilogue: eight neighbouring sums of row i, columns j.. -----------------------------------------------------------
 template <typename T> struct SlopeT;
-template <> struct SlopeT<bf16_t> { typedef f16_t type; };
-template <> struct SlopeT<float> { typedef float type; };
+template <> struct SlopeT<bf16_t> { typedef f16_t type; static constexpr float ONE = 0x1p14f; };      // how a slope of 1 is kept
+template <> struct SlopeT<float> { typedef float type; static constexpr float ONE = 1.f; };
 // Rows of any length and stride: 16-byte accesses that are aligned to an element only, which this machine's global memory
 // instructions take (f32 1001 x 515 x 1037 with SiLU, slopes and a residual: 37.5 us by elements, 32.8 so;
 // bf16 16383 x 1024 x 4095 with GELU, slopes and a residual 385, 245).
@@ -152,7 +156,7 @@ template <typename T> __device__ __forceinline__ void la_finish1(const GemmParam
   float s = 1.f;
   x += bias;
   la_act<T, 1>(&x, p.act, &s);
-  if (p.slope) ((S*)p.slope)[o] = (S)s;
+  if (p.slope) ((S*)p.slope)[o] = (S)(s * SlopeT<T>::ONE);
   if (p.res) x += (float)((const T*)p.res)[(int64_t)i * p.ldres + j];
   if (p.c_f32) ((float*)p.c)[o] = x; else ((T*)p.c)[o] = (T)x;
 }
@@ -192,7 +196,11 @@ template <typename T> __device__ __forceinline__ void la_finish8(const GemmParam
     for (int e = 0; e < 8; ++e) v[e] += bias[e];
     if (p.act != VG_ACT_NONE) {
       la_act<T, 8>(v, p.act, s);
-      if (p.slope) put8((S*)p.slope + o, s);
+      if (p.slope) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] *= SlopeT<T>::ONE;
+        put8((S*)p.slope + o, s);
+      }
     }
     if (p.res) {
 #pragma unroll
@@ -605,7 +613,7 @@ __global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, co
           for (int e = 0; e < 8; ++e) t[e] = j + e < n ? (float)slope[o + e] : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] *= t[e];
+        for (int e = 0; e < 8; ++e) g[e] *= t[e] * (1.f / SlopeT<T>::ONE);
         if constexpr (WHOLE) put8(dz + o, g);
         else {
 #pragma unroll
