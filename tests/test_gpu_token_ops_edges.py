@@ -192,3 +192,26 @@ def test_small_slopes_beside_bf16(act, rows):
     within(dx, slope, slope.abs() * (2.0 ** -11 + 2.0 ** -8 + rel) * 1.001 + 2.0 ** -39, "slope")
     if act == "sigmoid":
         assert bool((dx[z > -26] > 0)[:100].all())
+
+
+# ---------------------------------------------------------------------------------------------- forward-mode derivatives
+def test_tangents_are_refused_on_the_gpu():
+    """Also where the gradient that comes into a backward pass carries one."""
+    import torch.autograd.forward_ad as fwd
+    from vae_gan_amd import ops
+    x, w, b = torch.randn(4, 8, device="cuda"), torch.ones(8, device="cuda"), torch.zeros(8, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    calls = [lambda a: ops.layer_norm(a, w, b), lambda a: ops.linear_act(a, torch.eye(8, device="cuda"), b, 3), lambda a: ops.token_logprobs(a, t)[0]]
+    with fwd.dual_level():
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(fwd.make_dual(x, torch.ones_like(x)))
+            xg = x.clone().requires_grad_()
+            y = call(xg)
+            dy = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, xg, dy)
+    for call in calls:
+        xg = x.clone().requires_grad_()
+        y = call(xg)
+        assert torch.isfinite(torch.autograd.grad(y, xg, torch.ones_like(y))[0]).all()

@@ -2,7 +2,7 @@
 // vae_gan_amd/_vgtorch.so.  In C++ because these operators are called many times a step on small tensors: a Python autograd
 // function costs some 20 us of host time forward and 45 backward around kernels of 5 to 20 us, these 6 and 12.
 // Each checks its arguments, allocates its outputs and workspaces from torch's allocator and enqueues on the current stream
-// of its tensors' device.  None differentiates twice.
+// of its tensors' device.  None differentiates twice, carries forward-mode tangents: each refuses.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -32,6 +32,11 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(size_t n, const Tensor& like) { return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor(); }
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": cannot be differentiated twice (create_graph=True)");
+}
+// What launches kernels on memory cannot pass on a tangent (a result without one reads as a derivative of zero).
+void eager_only(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, ": has no forward-mode derivative (torch.autograd.forward_ad)");
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -73,6 +78,7 @@ struct LayerNorm : Function<LayerNorm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("layer_norm");
+    eager_only("layer_norm", {&g[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const c10::DeviceGuard guard(x.device());
@@ -94,6 +100,7 @@ struct LayerNorm : Function<LayerNorm> {
   }
 };
 Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, std::optional<int64_t> columns) {
+  eager_only("layer_norm", {&x, &weight, &bias});
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "layer_norm: no columns in a tensor of shape ", x.sizes());
   const int64_t c = columns.value_or(x.size(-1));
   TORCH_CHECK(c >= 1 && c <= x.size(-1), "layer_norm: c = ", c, " of ", x.size(-1), " columns");
@@ -140,6 +147,7 @@ struct LinearAct : Function<LinearAct> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list gs) {
     once("linear_act");
+    eager_only("linear_act", {&gs[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &slope = saved[2];
     const c10::DeviceGuard guard(x.device());
@@ -178,6 +186,7 @@ struct LinearAct : Function<LinearAct> {
 };
 Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_, int64_t act, const std::optional<Tensor>& residual_) {
   const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+  eager_only("linear_act", {&x, &weight, &bias, &residual});
   TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.numel() > 0,
               "linear_act: mat1 and mat2 shapes cannot be multiplied (", x.sizes(), " and ", weight.sizes(), " transposed)");
   vg_dtype("linear_act", x);
@@ -234,6 +243,7 @@ struct TokenLogprobs : Function<TokenLogprobs> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("token_logprobs");
+    eager_only("token_logprobs", {&g[0], &g[1]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &tokens = saved[1], &lse = saved[2], &entropy = saved[3];
     const c10::DeviceGuard guard(logits.device());
@@ -257,6 +267,7 @@ struct TokenLogprobs : Function<TokenLogprobs> {
 };
 variable_list token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t top, int64_t ignore) {
   constexpr int64_t most = 32;
+  eager_only("token_logprobs", {&logits});
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "token_logprobs: no logits in a tensor of shape ", logits.sizes());
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
   TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.sizes() == lead, "token_logprobs: tokens must be int64 ", lead, ", got ",
