@@ -33,3 +33,10 @@ def test_tangents_are_refused(ops):
                     call(*duals)
                 with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                     call(*duals)
+
+
+def test_traces_are_refused(ops):
+    """A trace would hold the allocation of the result and nothing that writes it."""
+    for call, args in calls(ops):
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(lambda *a: call(*a), tuple(args))

@@ -2,7 +2,8 @@
 // vae_gan_amd/_vgtorch.so.  In C++ because these operators are called many times a step on small tensors: a Python autograd
 // function costs some 20 us of host time forward and 45 backward around kernels of 5 to 20 us, these 6 and 12.
 // Each checks its arguments, allocates its outputs and workspaces from torch's allocator and enqueues on the current stream
-// of its tensors' device.  None differentiates twice, carries forward-mode tangents: each refuses.
+// of its tensors' device.  None differentiates twice, carries forward-mode tangents or can be traced: each refuses.
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -33,8 +34,10 @@ Tensor bytes(size_t n, const Tensor& like) { return n ? at::empty({(int64_t)n}, 
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": cannot be differentiated twice (create_graph=True)");
 }
-// What launches kernels on memory cannot pass on a tangent (a result without one reads as a derivative of zero).
+// What launches kernels on memory cannot pass on a tangent (a result without one reads as a derivative of zero), and a trace of it
+// would hold the allocation of its result alone.
 void eager_only(const char* what, std::initializer_list<const Tensor*> ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, ": cannot be traced (torch.jit.trace)");
   for (const Tensor* t : ts)
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, ": has no forward-mode derivative (torch.autograd.forward_ad)");
 }
