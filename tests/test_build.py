@@ -22,3 +22,10 @@ def test_the_library_needs_no_python_with_torch():
     assert "libvg_hip.so" in out and "torch_ops.cpp" not in out and "library alone" in out
     assert "torch_ops.cpp" not in dry("-B", "lib")
     assert "torch_ops.cpp" in dry("-B", "PYTHON=" + sys.executable)
+
+
+def test_a_changed_flag_reaches_every_object():
+    out = dry("-W", "Makefile", "lib")
+    for src in glob.glob(os.path.join(CSRC, "*.hip")):
+        name = os.path.basename(src)
+        assert any("-packed-fp32-ops" in line and f"-c {name} " in line for line in out.splitlines()), name
