@@ -40,3 +40,23 @@ def test_traces_are_refused(ops):
     for call, args in calls(ops):
         with pytest.raises(NotImplementedError, match="traced"):
             torch.jit.trace(lambda *a: call(*a), tuple(args))
+
+
+def test_other_operators_refuse_the_activations_of_linear_act(ops):
+    """GELU and SiLU are linear_act's; a convolution or BatchNorm asked for one must not run without an activation."""
+    from vae_gan_amd import lib as L
+    lib = L.load()
+    desc = None                                        # refused before it is read
+    one = 16
+    for act in (L.ACT_GELU, L.ACT_SILU, -1):
+        for name, rc in (("conv_fwd", lambda: lib.vg_conv_fwd(desc, one, one, None, one, None, act, 0, None)),
+                         ("conv_fwd_splitk", lambda: lib.vg_conv_fwd_splitk(desc, one, one, None, one, act, 2, one, None)),
+                         ("conv_dgrad", lambda: lib.vg_conv_dgrad(desc, one, one, None, one, None, act, 0, None)),
+                         ("thin_conv_fwd", lambda: lib.vg_thin_conv_fwd(desc, one, one, None, one, None, act, one, None)),
+                         ("conv1_fwd", lambda: lib.vg_conv1_fwd(desc, one, one, None, one, act, None)),
+                         ("bn_act_fwd", lambda: lib.vg_bn_act_fwd(one, None, one, one, one, 4, 64, 64, act, 0, None)),
+                         ("bn_bwd_reduce", lambda: lib.vg_bn_bwd_reduce(one, one, one, one, one, one, one, one, 4, 64, 64, 64, act, 0, None)),
+                         ("bn_bwd_apply", lambda: lib.vg_bn_bwd_apply(one, one, one, one, one, one, one, one, one, one, None, None, None, 0, None, 4, 4,
+                                                                      1.0, 64, 64, 64, act, 0, None)),
+                         ("act_bwd", lambda: lib.vg_act_bwd(one, one, one, 64, act, 0, None))):
+            assert rc() == -1 and name + ": activation" in L.last_error(), (name, act, L.last_error())

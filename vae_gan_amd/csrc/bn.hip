@@ -138,6 +138,7 @@ static int ew_blocks(int64_t work_items) {
 
 extern "C" int vg_bn_act_fwd(const void* x, const void* res, void* y, const float* scale, const float* shift, int64_t rows,
                              int cs, int c, int act, int dtype, void* stream) {
+  VG_ACT_CHECK("bn_act_fwd", act);
   VG_REQUIRE(x && y && scale && shift && rows > 0 && cs >= c, "bn_act_fwd: bad arguments");
   const int piece = dtype == VG_BF16 ? 8 : 4;
   VG_REQUIRE(cs % piece == 0 && cs / piece <= 256, "bn_act_fwd: channel stride %d unsupported", cs);
@@ -267,6 +268,7 @@ __global__ __launch_bounds__(256) void bn_bwd_reduce_kernel(const T* dout, const
 static int bn_bwd_reduce_launch(const void* dout, const void* y, const void* x, const float* mean, const float* invstd,
                                 const float* scale, const float* shift, double* sums, int64_t rows, int cs, int c, int cpad,
                                 int act, int dtype, void* dz, void* stream) {
+  VG_ACT_CHECK("bn_bwd_reduce", act);
   VG_REQUIRE(dout && x && mean && invstd && sums && rows > 0 && cs >= c && cpad >= c, "bn_bwd_reduce: bad arguments");
   VG_REQUIRE(y || (scale && shift), "bn_bwd_reduce: need y, or scale and shift to recompute the activation mask from x");
   const bool xmask = y == nullptr && act == VG_ACT_LRELU;
@@ -431,6 +433,7 @@ extern "C" int vg_bn_bwd_apply(const void* dout, const void* y, const void* x, c
                                const float* scale, const float* shift, const float* gamma, const double* sums, void* dx,
                                void* dres, float* dgamma, float* dbeta, int accumulate, float* dxsum, int64_t rows,
                                int64_t count, float dgb_scale, int cs, int c, int cpad, int act, int dtype, void* stream) {
+  VG_ACT_CHECK("bn_bwd_apply", act);
   VG_REQUIRE(dout && x && mean && invstd && sums && dx && rows > 0 && cs >= c && cpad >= c, "bn_bwd_apply: bad arguments");
   VG_REQUIRE(y || (scale && shift), "bn_bwd_apply: need y, or scale and shift to recompute the activation mask from x");
   VG_REQUIRE(y || act == VG_ACT_LRELU || act == VG_ACT_NONE, "bn_bwd_apply: y is required for this activation");
@@ -501,6 +504,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dout
 }
 
 extern "C" int vg_act_bwd(const void* dout, const void* y, void* dx, int64_t n, int act, int dtype, void* stream) {
+  VG_ACT_CHECK("act_bwd", act);
   VG_REQUIRE(dout && y && dx && n > 0, "act_bwd: bad arguments");
   const int piece = dtype == VG_BF16 ? 8 : 4;
   VG_REQUIRE(n % piece == 0, "act_bwd: element count %lld not a multiple of %d", (long long)n, piece);

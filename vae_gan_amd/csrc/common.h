@@ -30,6 +30,10 @@ void vg_set_error(const char* fmt, ...);
     }                                    \
   } while (0)
 
+// the activations that a convolution's or BatchNorm's kernels have (vg_linear_act_* check for theirs)
+#define VG_ACT_CHECK(what, act) \
+  VG_REQUIRE((act) >= VG_ACT_NONE && (act) <= VG_ACT_SIGMOID, "%s: activation %d (GELU and SiLU: vg_linear_act_* only)", what, act)
+
 #define VG_HIP(expr)                                                              \
   do {                                                                            \
     hipError_t e_ = (expr);                                                       \

@@ -2417,6 +2417,7 @@ static int conv_fwd_impl(const vg_conv_desc* d, const void* x, const void* w_pac
 
 extern "C" int vg_conv_fwd(const vg_conv_desc* d, const void* x, const void* w_packed, const float* bias, void* y,
                            double* stats, int act, int accumulate, void* stream) {
+  VG_ACT_CHECK("conv_fwd", act);
   return conv_fwd_impl(d, x, w_packed, bias, y, stats, act, accumulate, nullptr, nullptr, stream);
 }
 
@@ -2453,6 +2454,7 @@ extern "C" size_t vg_conv_splitk_ws_bytes(const vg_conv_desc* d) {
 
 extern "C" int vg_conv_fwd_splitk(const vg_conv_desc* d, const void* x, const void* w_packed, const float* bias, void* y,
                                   int act, int ksplit, void* ws, void* stream) {
+  VG_ACT_CHECK("conv_fwd_splitk", act);
   int rc = check_desc(d);
   if (rc) return rc;
   VG_REQUIRE(x && w_packed && y && ws, "conv_fwd_splitk: null pointer");
@@ -2532,6 +2534,7 @@ static int conv_dgrad_impl(const vg_conv_desc* d, const void* dy, const void* w_
 
 extern "C" int vg_conv_dgrad(const vg_conv_desc* d, const void* dy, const void* w_packed_t, const float* bias, void* dx,
                              double* stats, int act, int accumulate, void* stream) {
+  VG_ACT_CHECK("conv_dgrad", act);
   return conv_dgrad_impl(d, dy, w_packed_t, bias, dx, stats, act, accumulate, nullptr, nullptr, stream);
 }
 

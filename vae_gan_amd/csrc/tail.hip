@@ -224,6 +224,7 @@ static void conv1_fill(const vg_conv_desc* d, Conv1Params& p) {
 
 extern "C" int vg_conv1_fwd(const vg_conv_desc* d, const void* x, const float* w_oihw, const float* bias, void* y, int act,
                             void* stream) {
+  VG_ACT_CHECK("conv1_fwd", act);
   VG_REQUIRE(vg_conv1_supported(d), "conv1_fwd: not a supported one-channel 4x4 stride-1 conv");
   VG_REQUIRE(x && w_oihw && y, "conv1_fwd: null pointer");
   Conv1Params p;

@@ -628,6 +628,7 @@ static int launch_thin_out3(ThinParams& p, hipStream_t st) {
 
 extern "C" int vg_thin_conv_fwd(const vg_conv_desc* d, const void* x, const float* w_oihw, const float* bias, void* y,
                                 double* stats, int act, void* ws, void* stream) {
+  VG_ACT_CHECK("thin_conv_fwd", act);
   const int kind = vg_thin_conv_supported(d);
   VG_REQUIRE(kind != 0, "thin_conv_fwd: not a supported thin layer");
   VG_REQUIRE(x && w_oihw && y && ws, "thin_conv_fwd: null pointer");
