@@ -436,12 +436,18 @@ int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* tokens
 /* AdamW (decoupled weight decay) over a flat buffer of n elements, n a multiple of 256, every tensor begun at a multiple of 256:
  *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  p = p (1 - lr wd) - lr / (1-b1^step) * m / (sqrt(v / (1-b2^step)) + eps)
  * g is multiplied by grad_scale first.  decay: [n / 256] bytes, 0 = the block's tensor is not decayed; NULL: all are.
- * The 8-bit form keeps m and sqrt(v) as e4m3 codes with one f32 scale per 256 elements (largest magnitude / 448). */
+ * The 8-bit forms keep m and sqrt(v) as e4m3 codes with one f32 scale per 256 elements (largest magnitude / 448).  _step rounds
+ * them to nearest: a moment that changes by less than half a code (3 to 6 %) a step stays where it is within its 256.  _dithered_step
+ * rounds up with the probability of what is cut off, so moments follow on average; its random bits depend on the element's place,
+ * its gradient and `step` alone. */
 int vg_adamw_step(float* p, const float* g, float* m, float* v, const unsigned char* decay, int64_t n, double lr, double beta1, double beta2,
                   double eps, double weight_decay, int step, float grad_scale, void* stream);
 int vg_adamw8_step(float* p, const float* g, void* m_codes, float* m_scale, void* r_codes, float* r_scale, const unsigned char* decay,
                    int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay, int step, float grad_scale,
                    void* stream);
+int vg_adamw8_dithered_step(float* p, const float* g, void* m_codes, float* m_scale, void* r_codes, float* r_scale,
+                            const unsigned char* decay, int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay,
+                            int step, float grad_scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -215,3 +215,95 @@ def test_tangents_are_refused_on_the_gpu():
         xg = x.clone().requires_grad_()
         y = call(xg)
         assert torch.isfinite(torch.autograd.grad(y, xg, torch.ones_like(y))[0]).all()
+
+
+# ---------------------------------------------------------------------------------------------- AdamW in 8 bits over many steps
+def builder_optimizer():
+    """The generator's optimizer of `--optimizer adamw8bit`, over 64 blocks of 256 elements."""
+    from types import SimpleNamespace
+    from vae_gan_amd.train import build_optimizers
+    model = torch.nn.Module()
+    model.encoder, model.decoder, model.discriminator = (torch.nn.Linear(256, 64, bias=False).cuda() for _ in range(3))
+    model.decoder.weight.requires_grad_(False)
+    return build_optimizers(model, SimpleNamespace(optimizer="adamw8bit", lr=1e-4, beta1=0.9, beta2=0.999, weight_decay=0.0))[0]
+
+
+def test_adamw_8bit_second_moments_follow_inside_a_block():
+    """Half of every block's gradients are three times as large as the state that the run starts from.  1000 steps later each half's
+    moments are right on average.  A step changes a root by 0.0005 |g^2 / v - 1| of itself, 0.0005 on average, f = 0.004 to 0.008 of
+    a code's step of 0.06 to 0.125: rounding adds a variance of f (1 - f) squared steps and the decay of 0.0005 a step takes it
+    back, so the deviation is sqrt(f / 0.001) steps, 17 to 25 %, and, the root being what is rounded, half its square, at most
+    3 %, too much on average.  The median of 8192 elements is off by 0.25 * 1.25 / 90 = 0.0035, four times that is 0.014; 5 %
+    covers both.  Without the changes' share of the rounding the medians are 0.94 and 2.3."""
+    opt = builder_optimizer()
+    g = gen(7)
+    size = torch.exp(0.7 * torch.randn(64, 256, device="cuda", generator=g))
+    scale = size.amax(1, keepdim=True) / 448
+    opt.root_sq.copy_((size / scale).to(torch.float8_e4m3fn).view(-1))
+    opt.root_sq_scale.copy_(scale[:, 0])
+    v = (size / scale).to(torch.float8_e4m3fn).double().mul(scale.double()).square()
+    size[:, :128] *= 3
+    for _ in range(1000):
+        grad = size * torch.randn(64, 256, device="cuda", generator=g)
+        v = 0.999 * v + 0.001 * grad.double().square()
+        opt.flat_g.copy_(grad.view(-1))
+        opt.step()
+    ratio = opt.root_sq.float().view(64, 256) * opt.root_sq_scale[:, None] / v.sqrt()
+    for half in (ratio[:, :128], ratio[:, 128:]):
+        assert abs(float(half.median()) - 1) <= 0.05 and float(half.std()) <= 0.3, (float(half.median()), float(half.std()))
+
+
+def test_adamw_8bit_first_moments_reach_a_steady_gradient():
+    """Gradients of 1 beside one of 10 in each block, whose moment is there already and sets the scale: m goes to 1 (rounded to
+    nearest it stops at 0.71, where a tenth of what is left is less than half a step).  f = 0.1 (1 - m) steps, at most 0.1 near the
+    end: a deviation of sqrt(0.1 / 0.2) steps of 6 to 12 %, below 0.09; the mean of 16320 elements is off by 0.0007, and the two
+    sides of 1 have steps of 1/16 and 1/8 in which the same deviation is not the same probability: 2 % covers it."""
+    opt = builder_optimizer()
+    opt.flat_g.fill_(1.0)
+    opt.flat_g[::256] = 10.0
+    opt.exp_avg[::256] = 448.0
+    opt.exp_avg_scale.fill_(10 / 448)
+    for _ in range(300):
+        opt.step()
+    m = (opt.exp_avg.float().view(64, 256) * opt.exp_avg_scale[:, None])[:, 1:]
+    assert abs(float(m.mean()) - 1) <= 0.02 and float(m.std()) <= 0.12, (float(m.mean()), float(m.std()))
+    assert float((m.mean(1) - 1).abs().max()) <= 0.02 + 5 * 0.09 / 16      # 255 elements a block
+
+
+def test_adamw_8bit_stochastic_rounding_takes_either_neighbour():
+    """One step: each code is one of the two beside the exact value, and their mean is the exact value (a deviation of at most half a
+    step each: five standard errors of n elements, and 2^-16 for the 16 bits of chance).  Scales, parameters and updates are those
+    of rounding to nearest; the same step again gives the same bits."""
+    from test_gpu_token_ops import SHAPES, make_opt, states
+    opt, g = make_opt(8, shapes=SHAPES + [(300, 256)])
+    for _ in range(3):
+        opt.flat_g.copy_(torch.randn(opt.numel, device="cuda", generator=g) * torch.exp(2 * torch.randn(opt.numel, device="cuda", generator=g)))
+        for q, o in zip(opt.params, opt.offsets):
+            opt.flat_g[o + q.numel():(o + q.numel() + 255) // 256 * 256] = 0
+        opt.step()
+    m, v = states(opt)
+    sd, grad = opt.state_dict(), opt.flat_g.double()
+    two = []
+    for _ in range(2):
+        o, _ = make_opt(8, shapes=SHAPES + [(300, 256)], rounding="stochastic")
+        o.load_state_dict(sd)
+        o.flat_p.copy_(opt.flat_p), o.flat_g.copy_(opt.flat_g)
+        two.append(o)
+    for o in (opt, *two):
+        o.step()
+    a, b = two
+    for name in ("flat_p", "exp_avg_scale", "root_sq_scale"):
+        assert torch.equal(getattr(a, name), getattr(opt, name)), name
+    for name in ("exp_avg", "root_sq"):
+        assert torch.equal(getattr(a, name).view(torch.uint8), getattr(b, name).view(torch.uint8)), name
+    b1, b2 = opt.betas
+    for codes, scale, exact in ((a.exp_avg, a.exp_avg_scale, b1 * m + (1 - b1) * grad), (a.root_sq, a.root_sq_scale, (b2 * v + (1 - b2) * grad * grad).sqrt())):
+        q = (exact.view(-1, 256) / scale.double()[:, None]).view(-1)
+        q = torch.where(q.abs() < 2.0 ** -9, torch.zeros_like(q), q) if codes is a.root_sq else q      # raised to 2^-9
+        got = torch.where(q == 0, torch.zeros_like(q), codes.double())
+        step = torch.exp2(torch.floor(torch.log2(q.abs().clamp_min(2.0 ** -6))) - 3)
+        off = (got - q) / step
+        assert float(off.abs().max()) <= 1 + 2.0 ** -12
+        n = int((q != 0).sum())
+        assert abs(float(off.sum()) / n) <= 5 * 0.5 / n ** 0.5 + 2.0 ** -15, float(off.sum()) / n
+        assert float((off.abs() > 0.55).float().mean()) > 0.1                                          # not to nearest

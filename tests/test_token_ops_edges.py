@@ -60,3 +60,18 @@ def test_other_operators_refuse_the_activations_of_linear_act(ops):
                                                                       1.0, 64, 64, 64, act, 0, None)),
                          ("act_bwd", lambda: lib.vg_act_bwd(one, one, one, 64, act, 0, None))):
             assert rc() == -1 and name + ": activation" in L.last_error(), (name, act, L.last_error())
+
+
+def test_adamw_rounding_refusals(ops):
+    from vae_gan_amd import lib as L
+    from vae_gan_amd.optim import FlatAdamW
+    p = [torch.nn.Parameter(torch.zeros(4, 4))]
+    with pytest.raises(ValueError, match="rounding"):
+        FlatAdamW(p, state_bits=8, rounding="down")
+    with pytest.raises(ValueError, match="rounding"):
+        FlatAdamW(p, state_bits=32, rounding="stochastic")
+    lib, one = L.load(), 16
+    assert lib.vg_adamw8_dithered_step(one, one, one + 1, one, one, one, None, 256, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 1.0, None) == -1
+    assert "adamw8_dithered_step: states must be 4-byte aligned" in L.last_error()
+    assert lib.vg_adamw8_dithered_step(one, one, one, one, one, one, None, 255, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 1.0, None) == -1
+    assert "multiple" in L.last_error()

@@ -11,7 +11,7 @@ Every reference flag keeps its name, type, default and meaning: ``--output_dir -
   --recon_target_policy {error,area} 'error' raises like beta_vae_gans/model.py:255; 'area' is shim D1
   --hier_decoder_policy {error,nearest}  'error' raises like hierarchical_vae_gan/model.py:261; 'nearest' is shim D2
   --optimizer {adam,adamw,adamw8bit} 'adam' is the reference's; 'adamw' decays weights by --weight_decay (default 0.01),
-                                     'adamw8bit' also keeps its moments in 8 bits
+                                     'adamw8bit' also keeps its moments in 8 bits, rounded stochastically
   --image_size N                     Config.image_size (the reference has no flag for it)
   --num_workers N                    Config.num_workers (PNG-decoding loader processes; the reference has no flag)
   --max_iters N                      stop every epoch after N iterations (smoke runs)
@@ -64,7 +64,7 @@ def build_parser(arch: str) -> argparse.ArgumentParser:
         p.add_argument('--hier_decoder_policy', choices=('error', 'nearest'), default='error',
                        help="'error' raises like the reference's decoder, 'nearest' chains the sub-blocks with nearest x2")
     p.add_argument('--optimizer', choices=('adam', 'adamw', 'adamw8bit'), default='adam',
-                   help='adam: the reference; adamw: decoupled weight decay; adamw8bit: the same with 8-bit states')
+                   help='adam: the reference; adamw: decoupled weight decay; adamw8bit: the same with 8-bit states, rounded stochastically')
     p.add_argument('--weight_decay', type=float, default=0.01, help='weight decay of adamw / adamw8bit (weights only)')
     p.add_argument('--image_size', type=int, default=None, help='Config.image_size (default: the config value, 256)')
     p.add_argument('--num_workers', type=int, default=None, help='Config.num_workers (default: the config value, 4)')

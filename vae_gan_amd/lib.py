@@ -137,6 +137,7 @@ SIGNATURES = {
     "vg_token_logprobs_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
     "vg_adamw_step": (_I, [_P, _P, _P, _P, _P, _L, _D, _D, _D, _D, _D, _I, _F, _P]),
     "vg_adamw8_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _D, _D, _D, _D, _D, _I, _F, _P]),
+    "vg_adamw8_dithered_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _D, _D, _D, _D, _D, _I, _F, _P]),
     "vg_augment_ws_bytes": (C.c_size_t, [_AP, _I, _I, _I]),
     "vg_augment_batch": (_I, [_AP, _I, _I, _I, _P, C.c_size_t, _P, _P]),
     "vg_codebook_usage": (_I, [_P, _L, _I, _I, _P, _P, _P]),

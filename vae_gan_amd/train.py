@@ -26,7 +26,7 @@ def build_optimizers(model, config):
         make = FlatAdam
     elif kind in ("adamw", "adamw8bit"):
         make = functools.partial(FlatAdamW, weight_decay=getattr(config, "weight_decay", 0.01), decay_filter=lambda p: p.dim() > 1,
-                                 state_bits=8 if kind == "adamw8bit" else 32)
+                                 **(dict(state_bits=8, rounding="stochastic") if kind == "adamw8bit" else {}))
     else:
         raise ValueError(f"config.optimizer must be 'adam', 'adamw' or 'adamw8bit', got {kind!r}")
     opt_g = make(list(model.encoder.parameters()) + list(model.decoder.parameters()), lr=config.lr,
