@@ -390,7 +390,7 @@ int vg_linear_dgrad(const float* gy, const float* w, float* dx, int b, int fin, 
  * backward pass.  w, b, dw, db f32; x, y, dy, dx in `dtype`.  rows < 2^31. */
 int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, int64_t ldy, float* stats, int64_t rows, int c,
                       int cs, float eps, int dtype, void* stream);
-/* dx, and dw / db (either may be NULL) through per-block partial sums in ws (vg_layer_norm_bwd_ws_bytes), added in a fixed
+/* dx (NULL: not wanted), and dw / db (either may be NULL) through per-block partial sums in ws (vg_layer_norm_bwd_ws_bytes), added in a fixed
  * order: the same bits on every run. */
 size_t vg_layer_norm_bwd_ws_bytes(int64_t rows, int c);
 int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* w, const float* stats, void* dx, int64_t lddx,

@@ -307,3 +307,28 @@ def test_adamw_8bit_stochastic_rounding_takes_either_neighbour():
         n = int((q != 0).sum())
         assert abs(float(off.sum()) / n) <= 5 * 0.5 / n ** 0.5 + 2.0 ** -15, float(off.sum()) / n
         assert float((off.abs() > 0.55).float().mean()) > 0.1                                          # not to nearest
+
+
+# ---------------------------------------------------------------------------------------------- gradients that nobody asked for
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("c", [41, 512, 5000, 9001])
+def test_layer_norm_without_a_gradient_of_x(c, dt):
+    """Parameters alone: the same bits as beside dx, and its memory less (workspaces are the same: up to 768 parts of 8 c bytes)."""
+    from vae_gan_amd import ops
+    g = gen(c)
+    rows = (8 << 20) // c
+    x, dy = torch.randn(rows, c, device="cuda", generator=g).to(dt), torch.randn(rows, c, device="cuda", generator=g).to(dt)
+    w, b = torch.randn(c, device="cuda", generator=g).requires_grad_(), torch.randn(c, device="cuda", generator=g).requires_grad_()
+
+    def grads(xs, wanted):
+        y = ops.layer_norm(xs, w, b)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = torch.autograd.grad(y, wanted, dy)
+        return out, torch.cuda.max_memory_allocated() - before
+    xg = x.detach().requires_grad_()
+    full, more = grads(xg, (xg, w, b))
+    (dw, db), less = grads(x, (w, b))
+    assert more - less >= x.numel() * x.element_size()
+    assert torch.equal(dw, full[1]) and torch.equal(db, full[2])

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void ln_fwd_long_kernel(const T* __restrict__ 
   for (int i = threadIdx.x; i < cs; i += 256) y[row * ldy + i] = (T)(i < c ? ((float)xr[i] - mu - rest) * r * w[i] + b[i] : 0.f);
 }
 
-// dx of the rows of this block (block-strided), and the block's partial sums of dw and db: part[block][2][c]
+// dx of the rows of this block (block-strided; null: not wanted), and the block's partial sums of dw and db: part[block][2][c]
 template <typename T, int VEC, int GL, int NV, bool PART>
 __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy, int64_t lddy,
                                                      const float* __restrict__ w, const float* __restrict__ stats,
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ x, in
     }
     // two LDS slots in turn: a wave can be one row ahead of the readers of the other pair
     const float mg = row_sum<GL>(sg, red, turn) * inv, mgx = row_sum<GL>(sgx, red, turn + 1) * inv;
-    if (live) {
+    if (live && dx) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * GL + gl) * VEC;
@@ -434,8 +434,8 @@ extern "C" int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int
                                  void* dx, int64_t lddx, float* dw, float* db, void* ws, int64_t rows, int c, int cs, int dtype,
                                  void* stream) {
   if (int rc = ln_check("layer_norm_bwd", rows, c, cs, ldx, lddy, dtype)) return rc;
-  VG_REQUIRE(lddx >= cs, "layer_norm_bwd: a row stride below the row's %d columns", cs);
-  VG_REQUIRE(rows > 0 && x && dy && w && stats && dx, "layer_norm_bwd: null pointer or no rows");
+  VG_REQUIRE(!dx || lddx >= cs, "layer_norm_bwd: a row stride below the row's %d columns", cs);
+  VG_REQUIRE(rows > 0 && x && dy && w && stats && (dx || dw || db), "layer_norm_bwd: null pointer or no rows");
   VG_REQUIRE((!dw && !db) || ws, "layer_norm_bwd: the parameter gradients need a workspace");
   hipStream_t st = (hipStream_t)stream;
   float* part = dw || db ? (float*)ws : nullptr;
@@ -447,10 +447,10 @@ extern "C" int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int
     parts = (int)vg_ceil_div(rows, per);
     const dim3 grid((unsigned)vg_ceil_div(c, 256), (unsigned)parts);
     if (dtype == VG_BF16) {
-      hipLaunchKernelGGL(ln_bwd_long_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, (const bf16_t*)x, ldx, (const bf16_t*)dy, lddy, w, stats, (bf16_t*)dx, lddx, c, cs);
+      if (dx) hipLaunchKernelGGL(ln_bwd_long_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, (const bf16_t*)x, ldx, (const bf16_t*)dy, lddy, w, stats, (bf16_t*)dx, lddx, c, cs);
       if (part) hipLaunchKernelGGL(ln_bwd_long_params_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)x, ldx, (const bf16_t*)dy, lddy, stats, part, rows, c, per);
     } else {
-      hipLaunchKernelGGL(ln_bwd_long_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, (const float*)x, ldx, (const float*)dy, lddy, w, stats, (float*)dx, lddx, c, cs);
+      if (dx) hipLaunchKernelGGL(ln_bwd_long_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, (const float*)x, ldx, (const float*)dy, lddy, w, stats, (float*)dx, lddx, c, cs);
       if (part) hipLaunchKernelGGL(ln_bwd_long_params_kernel<float>, grid, dim3(256), 0, st, (const float*)x, ldx, (const float*)dy, lddy, stats, part, rows, c, per);
     }
   }

@@ -87,7 +87,8 @@ struct LayerNorm : Function<LayerNorm> {
     const c10::DeviceGuard guard(x.device());
     const int64_t c = ctx->saved_data["c"].toInt(), cs = x.size(-1);
     const Rows r = rows_of(x), d = rows_of(g[0]);
-    Tensor dx = at::empty(x.sizes(), x.options()), dw, db, ws;
+    Tensor dx, dw, db, ws;
+    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
     if (ctx->needs_input_grad(1)) dw = at::empty({c}, w.options());
     if (ctx->needs_input_grad(2)) db = at::empty({c}, w.options());
     if (r.n == 0) {
