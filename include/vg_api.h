@@ -387,7 +387,7 @@ int vg_linear_dgrad(const float* gy, const float* w, float* dx, int b, int fin, 
 /* ---- token-wise operators of a model of the code indices (no counterpart in the reference, which stops at the index map) ----
  * Layer norm over the first c of cs columns; rows have a stride of ldx / ldy elements; columns c..cs-1 of y and dx are
  * written as zeros.  y = (x - mean) * rstd * w + b.  stats: [rows][2] f32 out (mean, 1/sqrt(var + eps)), NULL without a
- * backward pass.  w, b, dw, db f32; x, y, dy, dx in `dtype`.  rows < 2^31. */
+ * backward pass.  w, b, dw, db f32; x, y, dy, dx in `dtype`.  rows < 2^31, cs <= 2^30. */
 int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, int64_t ldy, float* stats, int64_t rows, int c,
                       int cs, float eps, int dtype, void* stream);
 /* dx (NULL: not wanted), and dw / db (either may be NULL) through per-block partial sums in ws (vg_layer_norm_bwd_ws_bytes), added in a fixed

@@ -75,3 +75,15 @@ def test_adamw_rounding_refusals(ops):
     assert "adamw8_dithered_step: states must be 4-byte aligned" in L.last_error()
     assert lib.vg_adamw8_dithered_step(one, one, one, one, one, one, None, 255, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 1.0, None) == -1
     assert "multiple" in L.last_error()
+
+
+def test_rows_beyond_the_range_of_the_kernels_indexes(ops):
+    """A row of 2^32 + 8 elements must not be taken for one of 8."""
+    from vae_gan_amd import lib as L
+    lib, one, most = L.load(), 16, 1 << 30
+    x = torch.empty(1, (1 << 32) + 8, device="meta")
+    with pytest.raises(RuntimeError, match="columns in a row"):
+        ops.layer_norm(x, torch.ones(8), torch.ones(8), c=8)
+    with pytest.raises(RuntimeError, match="logits in a row"):
+        ops.token_logprobs(x, torch.zeros(1, dtype=torch.int64))
+    assert lib.vg_layer_norm_fwd(one, 2 * most, one, one, one, 2 * most, None, 1, 8, most + 8, 1e-5, 0, None) == -1 and "stored" in L.last_error()

@@ -401,7 +401,7 @@ static int ln_dispatch(const LnArgs& a, int dtype, bool bwd, hipStream_t st) {
 
 static int ln_check(const char* what, int64_t rows, int c, int cs, int64_t ld0, int64_t ld1, int dtype) {
   VG_REQUIRE(dtype == VG_F32 || dtype == VG_BF16, "%s: dtype %d", what, dtype);
-  VG_REQUIRE(rows >= 0 && rows < (1LL << 31) && c >= 1 && cs >= c, "%s: %ld rows of %d columns, %d stored", what, (long)rows, c, cs);
+  VG_REQUIRE(rows >= 0 && rows < (1LL << 31) && c >= 1 && cs >= c && cs <= (1 << 30), "%s: %ld rows of %d columns, %d stored", what, (long)rows, c, cs);
   VG_REQUIRE(ld0 >= cs && ld1 >= cs, "%s: a row stride below the row's %d columns", what, cs);
   return VG_OK;
 }
