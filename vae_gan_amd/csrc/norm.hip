@@ -78,6 +78,11 @@ template <int GL> __device__ __forceinline__ float row_sum(float v, float* red, 
   }
   return v;
 }
+// a product as one f32, not contracted into the differences that take it: those of equal values have to be equal and short
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 // two sums with one barrier between them, in slots `slot` and `slot` + 1
 template <int GL> __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int slot) {
   a = lane_sum<GL>(a);
@@ -97,7 +102,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, in
   __shared__ float red[24];
   constexpr int RPB = 256 / GL;
   const int gl = threadIdx.x % GL;
-  const float n = (float)c;
+  const float n = (float)c, inv = 1.f / n;
   float wv[NV][VEC], bv[NV][VEC];                    // zero in the padding: y comes out as 0 there
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -128,7 +133,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, in
         s += v[i][e];
       }
     fetch(row + step);
-    const float mu = row_sum<GL>(s, red, turn) / n;
+    const float mu = rounded_product(row_sum<GL>(s, red, turn), inv);
     float q = 0.f, rest = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -139,8 +144,8 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, in
         q += v[i][e] * v[i][e];
       }
     row_sum2<GL>(rest, q, red, turn + 1);
-    rest /= n;
-    const float r = 1.f / sqrtf(fmaxf(q / n - rest * rest, 0.f) + eps);
+    rest /= n;                                       // divided: exact for a constant row
+    const float r = 1.f / sqrtf(fmaxf((q - rest * rest * n) * inv, 0.f) + eps);
     if (!live) continue;
     if (stats && gl == 0) { stats[2 * row] = mu + rest; stats[2 * row + 1] = r; }
 #pragma unroll
