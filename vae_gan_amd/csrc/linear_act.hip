@@ -19,6 +19,16 @@
 typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef _Float16 f16_t;
 
+// e^x for x <= 0.  Beside f32 results the part of x log2 e that its f32 product leaves out is applied to the machine's base-2
+// exponential (off by an ulp, as its reciprocal is), which is then off by 3 u instead of |x| u; beside bf16 that does not show.
+// Below 2^-126 it is 0.
+template <typename T> __device__ __forceinline__ float la_exp(float x) {
+  constexpr float L = 1.4426950408889634f, L_REST = 1.92596299e-8f;      // log2 e
+  if constexpr (sizeof(T) == 2) return __expf(x);
+  x = x < -128.f ? -128.f : x;                       // a NaN stays one, and -inf does not make one
+  const float h = x * L, rest = fmaf(x, L_REST, fmaf(x, L, -h)), e = __builtin_amdgcn_exp2f(h);
+  return fmaf(e, rest * 0.6931471805599453f, e);
+}
 // Phi(-|x|) = e^(-x^2/2) t P(t) with t = 1 / (1 + p |x|), and that exponential, which the density needs too.  P is fitted to the
 // smallest relative error over |x| <= 13.5 (e^(-x^2/2) is 0 in f32 from there on), so z Phi(z) keeps its leading digits in the
 // negative tail: 3.7e-6 of Phi with six coefficients, for results in bf16 (2^-9), 6.1e-8 with eight, for f32, where x^2 is
@@ -28,21 +38,20 @@ template <typename T> __device__ __forceinline__ float la_phi(float x, float& e)
   const float a = fabsf(x), h = x * x;
   if constexpr (sizeof(T) == 2) {
     const float t = __builtin_amdgcn_rcpf(1.f + 0.307628282f * a);
-    e = __expf(-0.5f * h);
+    e = la_exp<T>(-0.5f * h);
     return e * t * (0.122990536f + t * (0.118537826f + t * (0.137324485f + t * (0.00529493169f + t * (0.191671309f + t * -0.0758208932f)))));
   } else {
-    const float t = 1.f / (1.f + 0.305121229f * a), low = h < __builtin_inff() ? fmaf(x, x, -h) : 0.f;
-    e = expf(-0.5f * h);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.305121229f * a), low = h < __builtin_inff() ? fmaf(x, x, -h) : 0.f;
+    e = la_exp<T>(-0.5f * h);
     e -= e * 0.5f * low;
     return e * t * (0.121686477f + t * (0.122538544f + t * (0.103320019f + t * (0.121442011f + t * (-0.0387208932f +
            t * (0.186413127f + t * (-0.153564337f + t * 0.0368851234f)))))));
   }
 }
 // p = 1 / (1 + e^-x) and q = 1 - p, both from e^-|x| in (0, 1]: neither is a difference, so p's slope p q keeps its leading
-// digits on either side.  Results in f32 take the library's exponential and a division (the matrix cores bind there), results in
-// bf16 the machine's base-2 exponential (|x| 2^-24 of itself) and reciprocal.
+// digits on either side.
 template <typename T> __device__ __forceinline__ void la_logistic(float x, float& p, float& q) {
-  const float e = sizeof(T) == 2 ? __expf(-fabsf(x)) : expf(-fabsf(x)), t = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+  const float e = la_exp<T>(-fabsf(x)), t = __builtin_amdgcn_rcpf(1.f + e);
   p = x < 0.f ? e * t : t;
   q = x < 0.f ? t : e * t;
 }
