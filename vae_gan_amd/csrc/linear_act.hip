@@ -9,8 +9,8 @@
 // All three products are C[i][j] = sum_k A(i, k) B(j, k), each operand either with k contiguous (x, W, dz in the first two)
 // or with i / j contiguous (W in dx = dz W, both in dW): a tile of the first kind is read from LDS with 16-byte reads, one of
 // the second with transposing reads, so nothing is transposed in memory.
-// Bound by the matrix cores where the sizes fill the chip (bf16 16384 x 1024 x 4096: forward 131 us without an activation, dx 124,
-// dW 110 and 13 to join four parts: 1050, 1110 and 1120 TFLOP/s), by launches and latency below some 10 GFLOP.
+// Bound by the matrix cores where the sizes fill the chip (bf16 16384 x 1024 x 4096: forward 152 us without an activation, dx 122,
+// dW 117 and 14 to join four parts: 900, 1130 and 1170 TFLOP/s), by launches and latency below some 10 GFLOP.
 #include <type_traits>
 
 #include "common.h"
@@ -32,7 +32,7 @@ template <typename T> __device__ __forceinline__ float la_exp(float x) {
 // Phi(-|x|) = e^(-x^2/2) t P(t) with t = 1 / (1 + p |x|), and that exponential, which the density needs too.  P is fitted to the
 // smallest relative error over |x| <= 13.5 (e^(-x^2/2) is 0 in f32 from there on), so z Phi(z) keeps its leading digits in the
 // negative tail: 3.7e-6 of Phi with six coefficients, for results in bf16 (2^-9), 6.1e-8 with eight, for f32, where x^2 is
-// carried in two parts as well.  A library erfc costs four times the instructions, and 67 M of them took as long as the
+// carried in two parts as well.  A library erf costs four times the instructions, and 67 M of them took as long as the
 // product of 16384 x 1024 x 4096 itself.
 template <typename T> __device__ __forceinline__ float la_phi(float x, float& e) {
   const float a = fabsf(x), h = x * x;
@@ -594,8 +594,9 @@ template <typename T> __global__ __launch_bounds__(256) void la_pack_kernel(cons
 
 // dz = dy slope (dz = dy without one) and partial column sums of the unrounded dz: part[row chunk][n].
 // A block is 32 column groups of 8 (512 bytes of a row) by 8 rows, so 16-byte accesses and runs of memory; bound by one read
-// of dy and slope and one write of dz.  Neither of the two is read again, so they do not take the cache from dz, which both
-// products read next (bf16 16384 x 1024 x 4096, forward + backward: 528 us with ordinary loads, 500 so).
+// of dy and slope and one write of dz.  The backward pass reads neither of the two again (dy may be, as the residual's gradient),
+// so they do not take the cache from dz, which both products read next (bf16 16384 x 1024 x 4096, forward + backward: 528 us with
+// ordinary loads, 500 so).
 template <typename T>
 __global__ __launch_bounds__(256) void la_dz_kernel(const T* __restrict__ dy, const typename SlopeT<T>::type* __restrict__ slope, T* __restrict__ dz,
                                                     float* __restrict__ part, int m, int n, int rows_per) {

@@ -2,8 +2,8 @@
 //   m = max x, s = sum e^(x-m), u = sum e^(x-m) (x-m):  logp = (x_t - m) - ln s,  H = ln s - u / s
 //   dx_j = dlogp ([j = t] - p_j) - dH p_j (ln p_j + H),  p_j = e^(x_j - lse)
 // Bound by memory: the forward reads the logits once, keeping (m, s, u) as running values that are rescaled when a larger
-// maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 71 and
-// 84 us, 805 MB at 5.2 TB/s, where the logits come from memory).  Sums are f32; exponents are of x - m <= 0.
+// maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 51 and
+// 83 us, 805 MB at 6.0 TB/s, a part of the logits from the last-level cache).  Sums are f32; exponents are of x - m <= 0.
 // Masked logits (-inf) have p = 0, so by the formula no gradient, except a masked token in a row that allows others: logp -inf,
 // and dlogp at its place.  A row of nothing but -inf has no distribution: logp -inf, H 0, gradient 0.  A
 // NaN or +inf in a row makes its logp, H and gradient NaN.  tokens[r] == ignore: logp 0 and no gradient through logp; any
@@ -163,7 +163,7 @@ template <typename T> __device__ __forceinline__ float token_logit(const LpParam
 
 // ---- rows that fit a wave's registers ------------------------------------------------------------------------------------
 // lane l holds 16-byte accesses l, l + 64, ..., aligned to an element only (the machine's global memory instructions take that)
-// GL lanes share a row (short rows: several to a wave; 65536 x 128 bf16: 18 us with a wave each, 6 with 16 lanes)
+// GL lanes share a row (short rows: several to a wave; 65536 x 128 bf16: 18 us with a wave each, 7 with 16 lanes)
 template <int GL, typename V, typename F> __device__ __forceinline__ V group_fold(V v, F f) {
 #pragma unroll
   for (int o = GL / 2; o > 0; o >>= 1) v = f(v, (V)__shfl_xor(v, o, 64));
@@ -561,8 +561,8 @@ template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
 #undef LP_CASE
     return;
   }
-  // Many rows: a wave each, which leaves no barrier between loads and sums, two accesses a batch (16384 x 8192 bf16: 52 us,
-  // 5.1 TB/s; a batch of four 72, since its registers halve the waves).  Few: a block each, with as many accesses in a batch
+  // Many rows: a wave each, which leaves no barrier between loads and sums, two accesses a batch (16384 x 8192 bf16: 51 us,
+  // 5.2 TB/s; a batch of four 72, since its registers halve the waves).  Few: a block each, with as many accesses in a batch
   // as a unit has for each thread.
   const int64_t units = p.rows * p.splits, per = vg_ceil_div(p.chunk < p.vocab ? p.chunk : p.vocab, 256 * Elt<T>::PIECE);
   if (units >= LP_WAVE_UNITS) hipLaunchKernelGGL((lp_row_kernel<T, 2, 64>), dim3((unsigned)vg_ceil_div(units, 4)), dim3(256), 0, st, p);
@@ -597,8 +597,8 @@ extern "C" int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int6
   if (rows == 0) return VG_OK;
   VG_REQUIRE(logits && tokens && lse && entropy && dx && lddx >= vocab, "token_logprobs_bwd: null pointer or a short row stride");
   LpBwdParams p = {logits, ldx, tokens, ignore, lse, entropy, dlogp, dent, dx, lddx, rows, vocab, 1, 0};
-  // up to a wave per row while the row is short (65536 x 128 bf16: 24 us with a wave, 9 with 16 lanes); otherwise blocks,
-  // each with at most 32 KB of a row
+  // up to a wave per row while the row is short (65536 x 128 bf16: 24 us with a wave, 10 with 16 lanes); otherwise blocks,
+  // each with at most 16384 elements of a row
   int tpr = vocab <= 4096 ? 64 : 256;
   while (tpr > 8 && vocab <= tpr / 2 * (16 / vg_elt_size(dtype))) tpr /= 2;
   p.chunk = tpr <= 64 ? (int)(vg_ceil_div(vocab, 8) * 8) : (1 << 14);

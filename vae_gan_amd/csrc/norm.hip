@@ -8,14 +8,14 @@
 // variance is that of the centred values (no cancellation of sum(x^2) - mu^2) at no second read.  All sums are f32; the mean of
 // the centred values, which is what the first mean's rounding left in them, is taken off them again: constant rows are exactly
 // centred and y = b, where a mean one step off would be raised by r, up to 316 at eps = 1e-5.
-// 16384 x 512 bf16: forward 10 us (3.4 TB/s), backward 13 us (3.9 TB/s) and 3.5 us for the column sums; 65536 x 128 f32 forward
-// 13.5 us (5.0 TB/s), where the launch's own few us weigh less.
+// 16384 x 512 bf16: forward 10.3 us (3.3 TB/s; 9.4 without the second mean), backward 13.2 us (3.8 TB/s) and 3.8 us for the column
+// sums; 65536 x 128 f32 forward 14.8 us (4.5 TB/s; 13.6), where the launch's own few us weigh less.
 #include "common.h"
 #include "rows.h"
 
 // VEC elements as loaded, so that the next row can be on its way while this one is worked on.  Accesses are aligned to an element
 // only (rows of any stride; the machine's global memory instructions take that).  PART: the last one of a row may have n < VEC
-// elements; whole rows do not pay for that (1024 x 8192 f32 forward: 16.6 us with, 13.0 without; x 8191 by elements: 26, so 17).
+// elements; whole rows do not pay for that (1024 x 8192 f32 forward: 17.1 us with, 13.4 without; x 8191 by elements: 26, so 17.1).
 template <typename T, int VEC, bool PART> struct Raw {
   typedef T vt __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   T __attribute__((ext_vector_type(VEC))) v;

@@ -1279,7 +1279,8 @@ def attention(q, k, v, x, gamma):
 
 # ----------------------------------------------------------------------------------------------
 # token-wise operators of a model of the code indices (csrc/norm.hip, linear_act.hip, logprobs.hip; autograd and argument
-# checks in csrc/torch_ops.cpp)
+# checks in csrc/torch_ops.cpp).  None differentiates twice, carries forward-mode tangents or can be traced by torch.jit: each
+# raises then.
 # ----------------------------------------------------------------------------------------------
 def _on_device(what: str, x: torch.Tensor):
     """A context in which launches go to the current stream of ``x``'s GPU."""
@@ -1299,7 +1300,8 @@ def linear_act(x, weight, bias=None, act: int = L.ACT_NONE, residual=None):
     f32 with everything after the sum in the product's epilogue.  ``weight`` [out, in] in ``x``'s dtype, or an f32 master
     weight for bf16 ``x`` (rounded to bf16 for the products; its gradient is f32).  ``bias`` [out] in ``x``'s dtype or f32;
     ``residual`` in ``x``'s dtype and the result's shape.  ``act``: ``L.ACT_NONE``, ``ACT_LRELU`` (0.2), ``ACT_SIGMOID``,
-    ``ACT_GELU`` (z Phi(z)) or ``ACT_SILU``."""
+    ``ACT_GELU`` (z Phi(z)) or ``ACT_SILU``.  Beside bf16, slopes of the activation below 2^-39 give no gradient (a sigmoid beyond
+    z = +-26), and its product with the incoming gradient is rounded to bf16 before the products of the backward pass."""
     return L.native().linear_act(x, weight, bias, act, residual)
 
 
