@@ -387,7 +387,8 @@ int vg_linear_dgrad(const float* gy, const float* w, float* dx, int b, int fin, 
 /* ---- token-wise operators of a model of the code indices (no counterpart in the reference, which stops at the index map) ----
  * Layer norm over the first c of cs columns; rows have a stride of ldx / ldy elements; columns c..cs-1 of y and dx are
  * written as zeros.  y = (x - mean) * rstd * w + b.  stats: [rows][2] f32 out (mean, 1/sqrt(var + eps)), NULL without a
- * backward pass.  w, b, dw, db f32; x, y, dy, dx in `dtype`.  rows < 2^31, cs <= 2^30. */
+ * backward pass.  w, b, dw, db f32; x, y, dy, dx in `dtype`.  rows < 2^31, cs <= 2^24
+ * (beyond 8192 columns also rows < 2^24). */
 int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, int64_t ldy, float* stats, int64_t rows, int c,
                       int cs, float eps, int dtype, void* stream);
 /* dx (NULL: not wanted), and dw / db (either may be NULL) through per-block partial sums in ws (vg_layer_norm_bwd_ws_bytes), added in a fixed
@@ -399,7 +400,7 @@ int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
 /* y = act(x W^T + bias) + res: x [m][k] (row stride ldx), w [n][k] in w_dtype (`dtype`, or VG_F32: rounded to `dtype` for the
  * products), y [m][n]; bias [n] in bias_dtype (`dtype` or VG_F32) or NULL; res [m][n] (row stride ldres) or NULL.  slope: NULL, or
  * [m][n] for act'(x W^T + bias), which vg_linear_act_dz takes (f16 of 2^14 times it for VG_BF16, f32 of itself for VG_F32).
- * f32 accumulation.  n, k < 2^20.  ws: the bytes that the _ws_bytes function names for the same operands (NULL for 0), aligned to 256. */
+ * f32 accumulation.  n, k < 2^20, m < 2^30 - 64, and m n and m k < 2^36 (one launch).  ws: the bytes that the _ws_bytes function names for the same operands (NULL for 0), aligned to 256. */
 size_t vg_linear_act_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int w_dtype, int64_t m, int64_t n, int64_t k, int dtype);
 int vg_linear_act_fwd(const void* x, int64_t ldx, const void* w, int w_dtype, const void* bias, int bias_dtype, const void* res,
                       int64_t ldres, void* y, void* slope, void* ws, int64_t m, int64_t n, int64_t k, int act, int dtype, void* stream);
@@ -425,7 +426,7 @@ const char* vg_last_linear_act_kernel(void);
  * masked: no probability and no gradient, except that a masked token in a row that allows others (logp -inf) gets dlogp at its place;
  * a row of only -inf gives logp -inf, entropy 0, gradient 0; NaN or +inf in a row gives NaN (a NaN ranks as -inf among the
  * alternatives).  tokens[r] == ignore: logp 0 and no gradient through it; another token outside [0, vocab): logp NaN, no gradient
- * through it.  ws: vg_token_logprobs_ws_bytes (0: none needed). */
+ * through it.  rows < 2^29 and rows vocab < 2^33 (one launch).  ws: vg_token_logprobs_ws_bytes (0: none needed). */
 size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top);
 int vg_token_logprobs_fwd(const void* logits, int64_t ldx, const int64_t* tokens, int64_t ignore, int64_t rows, int vocab, int top,
                           float* logp, float* entropy, float* lse, float* top_logp, int64_t* top_at, void* ws, int dtype, void* stream);

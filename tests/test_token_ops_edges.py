@@ -87,3 +87,19 @@ def test_rows_beyond_the_range_of_the_kernels_indexes(ops):
     with pytest.raises(RuntimeError, match="logits in a row"):
         ops.token_logprobs(x, torch.zeros(1, dtype=torch.int64))
     assert lib.vg_layer_norm_fwd(one, 2 * most, one, one, one, 2 * most, None, 1, 8, most + 8, 1e-5, 0, None) == -1 and "stored" in L.last_error()
+
+
+def test_launches_of_too_many_workgroups_are_refused_by_name(ops):
+    """2^32 threads or more in one dimension do not launch: the message says which operator's, and nothing is run before it."""
+    from vae_gan_amd import lib as L
+    lib, one = L.load(), 16
+
+    def refused(rc, name):
+        assert rc == -1 and name in L.last_error() and "too many" in L.last_error(), (rc, L.last_error())
+    n = (1 << 31) - 1
+    refused(lib.vg_token_logprobs_fwd(one, 8, one, -100, n, 8, 0, one, one, None, None, None, None, 1, None), "token_logprobs_fwd")
+    refused(lib.vg_token_logprobs_fwd(one, 4096, one, -100, n, 4096, 0, one, one, None, None, None, None, 1, None), "token_logprobs_fwd")
+    refused(lib.vg_token_logprobs_bwd(one, 8, one, -100, one, one, one, one, one, 8, n, 8, 1, None), "token_logprobs_bwd")
+    refused(lib.vg_layer_norm_fwd(one, 9000, one, one, one, 9000, None, 1 << 24, 9000, 9000, 1e-5, 1, None), "layer_norm_fwd")
+    refused(lib.vg_layer_norm_bwd(one, 9000, one, 9000, one, one, one, 9000, one, one, one, 1 << 24, 9000, 9000, 1, None), "layer_norm_bwd")
+    refused(lib.vg_linear_act_fwd(one, 64, one, 1, None, 0, None, 0, one, None, None, (1 << 30) - 1, 1024, 64, 0, 1, None), "linear_act")

@@ -34,6 +34,10 @@ void vg_set_error(const char* fmt, ...);
 #define VG_ACT_CHECK(what, act) \
   VG_REQUIRE((act) >= VG_ACT_NONE && (act) <= VG_ACT_SIGMOID, "%s: activation %d (GELU and SiLU: vg_linear_act_* only)", what, act)
 
+// a launch has fewer than 2^32 threads in a dimension
+#define VG_GRID_CHECK(what, blocks, threads) \
+  VG_REQUIRE((int64_t)(blocks) * (threads) < (1LL << 32), "%s: %lld workgroups are too many for one launch", what, (long long)(blocks))
+
 #define VG_HIP(expr)                                                              \
   do {                                                                            \
     hipError_t e_ = (expr);                                                       \

@@ -736,7 +736,7 @@ template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S> s
   void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S>;
   VG_HIP(vg_lds_attr((const void*)kernel, lds));
   const int64_t blocks = vg_ceil_div(p.m, BM) * vg_ceil_div(p.n, BN) * p.splits;
-  VG_REQUIRE(blocks < (1LL << 31), "linear_act: %d x %d outputs are too many for one launch", p.m, p.n);
+  VG_GRID_CHECK("linear_act", blocks, 64 * WM * WN);
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WM * WN), lds, st, p);
   VG_LAUNCH_CHECK();
   return VG_OK;

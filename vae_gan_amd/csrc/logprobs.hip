@@ -549,27 +549,32 @@ extern "C" size_t vg_token_logprobs_ws_bytes(int64_t rows, int vocab, int top) {
 }
 
 static const int64_t LP_WAVE_UNITS = 2048;          // two waves a SIMD
-template <typename T> static void lp_launch(const LpParams& p, hipStream_t st) {
+template <typename T> static int lp_launch(const LpParams& p, hipStream_t st) {
   if (lp_regs(p.vocab)) {
-#define LP_CASE(GL, NV)                                                                                                                       \
-  if (p.vocab <= GL * Elt<T>::PIECE * NV) {                                                                                                   \
-    hipLaunchKernelGGL((lp_wave_kernel<T, GL, NV>), dim3((unsigned)vg_ceil_div(p.rows, 256 / GL)), dim3(256), 0, st, p);                      \
-    return;                                                                                                                                   \
+#define LP_CASE(GL, NV)                                                                              \
+  if (p.vocab <= GL * Elt<T>::PIECE * NV) {                                                          \
+    const int64_t blocks = vg_ceil_div(p.rows, 256 / GL);                                            \
+    VG_GRID_CHECK("token_logprobs_fwd", blocks, 256);                                                \
+    hipLaunchKernelGGL((lp_wave_kernel<T, GL, NV>), dim3((unsigned)blocks), dim3(256), 0, st, p);    \
+    VG_LAUNCH_CHECK();                                                                               \
+    return VG_OK;                                                                                    \
   }
     LP_CASE(8, 1) LP_CASE(16, 1) LP_CASE(32, 1) LP_CASE(64, 1) LP_CASE(64, 2) LP_CASE(64, 4)
     if constexpr (sizeof(T) == 4) { LP_CASE(64, 8) }
 #undef LP_CASE
-    return;
   }
   // Many rows: a wave each, which leaves no barrier between loads and sums, two accesses a batch (16384 x 8192 bf16: 51 us,
   // 5.2 TB/s; a batch of four 72, since its registers halve the waves).  Few: a block each, with as many accesses in a batch
   // as a unit has for each thread.
   const int64_t units = p.rows * p.splits, per = vg_ceil_div(p.chunk < p.vocab ? p.chunk : p.vocab, 256 * Elt<T>::PIECE);
+  VG_GRID_CHECK("token_logprobs_fwd", units >= LP_WAVE_UNITS ? vg_ceil_div(units, 4) : units, 256);
   if (units >= LP_WAVE_UNITS) hipLaunchKernelGGL((lp_row_kernel<T, 2, 64>), dim3((unsigned)vg_ceil_div(units, 4)), dim3(256), 0, st, p);
   else if (per == 1) hipLaunchKernelGGL((lp_row_kernel<T, 1, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
   else if (per == 2) hipLaunchKernelGGL((lp_row_kernel<T, 2, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((lp_row_kernel<T, 4, 256>), dim3((unsigned)units), dim3(256), 0, st, p);
   if (p.splits > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)p.rows), dim3(256), 0, st, p);
+  VG_LAUNCH_CHECK();
+  return VG_OK;
 }
 
 extern "C" int vg_token_logprobs_fwd(const void* logits, int64_t ldx, const int64_t* tokens, int64_t ignore, int64_t rows, int vocab,
@@ -584,10 +589,7 @@ extern "C" int vg_token_logprobs_fwd(const void* logits, int64_t ldx, const int6
   lp_split(rows, vocab, &p.splits, &p.chunk);
   p.cand = (unsigned long long*)ws;                  // 8-byte values first
   p.part = (float*)((char*)ws + lp_keys_bytes(rows, p.splits, top));
-  if (dtype == VG_BF16) lp_launch<bf16_t>(p, (hipStream_t)stream);
-  else lp_launch<float>(p, (hipStream_t)stream);
-  VG_LAUNCH_CHECK();
-  return VG_OK;
+  return dtype == VG_BF16 ? lp_launch<bf16_t>(p, (hipStream_t)stream) : lp_launch<float>(p, (hipStream_t)stream);
 }
 
 extern "C" int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* tokens, int64_t ignore, const float* lse,
@@ -605,7 +607,7 @@ extern "C" int vg_token_logprobs_bwd(const void* logits, int64_t ldx, const int6
   p.splits = (int)vg_ceil_div(vocab, p.chunk);
   const int64_t units = rows * p.splits;
   const int64_t blocks = vg_ceil_div(units, 256 / tpr);
-  VG_REQUIRE(blocks < (1LL << 31), "token_logprobs_bwd: %ld rows of %d logits are too many for one launch", (long)rows, vocab);
+  VG_GRID_CHECK("token_logprobs_bwd", blocks, 256);
   const bool stream_out = rows * (int64_t)vocab * 2 * vg_elt_size(dtype) > LP_STREAM;
 #define LP_BWD(T, S) hipLaunchKernelGGL((lp_bwd_kernel<T, S>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, tpr)
   if (dtype == VG_BF16) { if (stream_out) LP_BWD(bf16_t, true); else LP_BWD(bf16_t, false); }

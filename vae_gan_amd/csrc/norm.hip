@@ -406,7 +406,7 @@ static int ln_dispatch(const LnArgs& a, int dtype, bool bwd, hipStream_t st) {
 
 static int ln_check(const char* what, int64_t rows, int c, int cs, int64_t ld0, int64_t ld1, int dtype) {
   VG_REQUIRE(dtype == VG_F32 || dtype == VG_BF16, "%s: dtype %d", what, dtype);
-  VG_REQUIRE(rows >= 0 && rows < (1LL << 31) && c >= 1 && cs >= c && cs <= (1 << 30), "%s: %ld rows of %d columns, %d stored", what, (long)rows, c, cs);
+  VG_REQUIRE(rows >= 0 && rows < (1LL << 31) && c >= 1 && cs >= c && cs <= (1 << 24), "%s: %ld rows of %d columns, %d stored", what, (long)rows, c, cs);
   VG_REQUIRE(ld0 >= cs && ld1 >= cs, "%s: a row stride below the row's %d columns", what, cs);
   return VG_OK;
 }
@@ -420,6 +420,7 @@ extern "C" int vg_layer_norm_fwd(const void* x, int64_t ldx, const float* w, con
   hipStream_t st = (hipStream_t)stream;
   LnArgs a = {x, nullptr, ldx, 0, ldy, w, b, y, stats, nullptr, rows, c, cs, eps};
   if (!ln_dispatch(a, dtype, false, st)) {
+    VG_GRID_CHECK("layer_norm_fwd", rows, 256);
     if (dtype == VG_BF16)
       hipLaunchKernelGGL(ln_fwd_long_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, (const bf16_t*)x, ldx, w, b, (bf16_t*)y, ldy, stats, c, cs, eps);
     else hipLaunchKernelGGL(ln_fwd_long_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, (const float*)x, ldx, w, b, (float*)y, ldy, stats, c, cs, eps);
@@ -447,6 +448,7 @@ extern "C" int vg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int
   LnArgs a = {x, dy, ldx, lddy, lddx, w, nullptr, dx, (float*)stats, part, rows, c, cs, 0.f};
   int parts = ln_dispatch(a, dtype, true, st);
   if (!parts) {
+    VG_GRID_CHECK("layer_norm_bwd", rows, 256);
     parts = rows < LN_LONG_PARTS ? (int)rows : LN_LONG_PARTS;
     const int64_t per = vg_ceil_div(rows, parts);
     parts = (int)vg_ceil_div(rows, per);

@@ -106,7 +106,7 @@ struct LayerNorm : Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, std::optional<int64_t> columns) {
   eager_only("layer_norm", {&x, &weight, &bias});
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "layer_norm: no columns in a tensor of shape ", x.sizes());
-  TORCH_CHECK(x.size(-1) <= (1 << 30), "layer_norm: ", x.size(-1), " columns in a row");
+  TORCH_CHECK(x.size(-1) <= (1 << 24), "layer_norm: ", x.size(-1), " columns in a row");
   const int64_t c = columns.value_or(x.size(-1));
   TORCH_CHECK(c >= 1 && c <= x.size(-1), "layer_norm: c = ", c, " of ", x.size(-1), " columns");
   for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"weight", weight}, {"bias", bias}})
