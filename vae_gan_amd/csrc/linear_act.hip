@@ -736,13 +736,11 @@ template <typename T, bool TA, bool TB, int WM, int WN, int MT, int NT, int S> s
   void (*kernel)(const GemmParams) = gemm_tile_kernel<T, TA, TB, WM, WN, MT, NT, S>;
   VG_HIP(vg_lds_attr((const void*)kernel, lds));
   const int64_t blocks = vg_ceil_div(p.m, BM) * vg_ceil_div(p.n, BN) * p.splits;
-  VG_GRID_CHECK("linear_act", blocks, 64 * WM * WN);
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WM * WN), lds, st, p);
   VG_LAUNCH_CHECK();
   return VG_OK;
 }
-template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int dtype, char* ws, hipStream_t st) {
-  const LaPlan pl = la_plan(p.m, p.n, p.k, dtype);
+template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, const LaPlan& pl, int dtype, char* ws, hipStream_t st) {
   p.splits = pl.splits;
   p.ktiles = pl.ktiles;
   p.ldp = (int)la_pitch(p.n);
@@ -765,13 +763,14 @@ template <typename T, bool TA, bool TB> static int la_gemm_t(GemmParams p, int d
 // C [m][n] = A B over k; a is stored [m][k] (ta: [k][m]), b [n][k] (tb: [k][n])
 static int la_gemm(GemmParams p, LaOperand a, bool ta, LaOperand b, bool tb, int dtype, void* ws, hipStream_t st) {
   VG_REQUIRE((uintptr_t)ws % 256 == 0 && (ws || la_ws(p.m, p.n, p.k, dtype, a, b) == 0), "linear_act: needs a workspace, aligned to 256 bytes");
+  const LaPlan pl = la_plan(p.m, p.n, p.k, dtype);
+  VG_GRID_CHECK("linear_act", vg_ceil_div(p.m, pl.tile) * vg_ceil_div(p.n, pl.tile) * pl.splits, pl.tile == 256 ? 512 : 256);
   LaOperand* both[2] = {&a, &b};
   char* w = la_pack(both, dtype, (char*)ws, st);
-  VG_LAUNCH_CHECK();
   p.a = a.p; p.lda = a.ld; p.b = b.p; p.ldb = b.ld;
   if (dtype == VG_BF16)
-    return ta ? la_gemm_t<bf16_t, true, true>(p, dtype, w, st) : tb ? la_gemm_t<bf16_t, false, true>(p, dtype, w, st) : la_gemm_t<bf16_t, false, false>(p, dtype, w, st);
-  return ta ? la_gemm_t<float, true, true>(p, dtype, w, st) : tb ? la_gemm_t<float, false, true>(p, dtype, w, st) : la_gemm_t<float, false, false>(p, dtype, w, st);
+    return ta ? la_gemm_t<bf16_t, true, true>(p, pl, dtype, w, st) : tb ? la_gemm_t<bf16_t, false, true>(p, pl, dtype, w, st) : la_gemm_t<bf16_t, false, false>(p, pl, dtype, w, st);
+  return ta ? la_gemm_t<float, true, true>(p, pl, dtype, w, st) : tb ? la_gemm_t<float, false, true>(p, pl, dtype, w, st) : la_gemm_t<float, false, false>(p, pl, dtype, w, st);
 }
 
 // Whether the few-rows kernel takes a forward product: its time is bound by one read of the weights from memory (3.9 TB/s) or
