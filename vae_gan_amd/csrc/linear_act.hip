@@ -9,8 +9,8 @@
 // All three products are C[i][j] = sum_k A(i, k) B(j, k), each operand either with k contiguous (x, W, dz in the first two)
 // or with i / j contiguous (W in dx = dz W, both in dW): a tile of the first kind is read from LDS with 16-byte reads, one of
 // the second with transposing reads, so nothing is transposed in memory.
-// Bound by the matrix cores where the sizes fill the chip (bf16 16384 x 1024 x 4096: forward 152 us without an activation, dx 122,
-// dW 117 and 14 to join four parts: 900, 1130 and 1170 TFLOP/s), by launches and latency below some 10 GFLOP.
+// Bound by the matrix cores where the sizes fill the chip (bf16 16384 x 1024 x 4096 in a training pass: forward 157 us without an
+// activation, dx 116, dW 114 and 14 to join four parts: 875, 1180 and 1200 TFLOP/s), by launches and latency below some 10 GFLOP.
 #include <type_traits>
 
 #include "common.h"

@@ -2,7 +2,7 @@
 //   m = max x, s = sum e^(x-m), u = sum e^(x-m) (x-m):  logp = (x_t - m) - ln s,  H = ln s - u / s
 //   dx_j = dlogp ([j = t] - p_j) - dH p_j (ln p_j + H),  p_j = e^(x_j - lse)
 // Bound by memory: the forward reads the logits once, keeping (m, s, u) as running values that are rescaled when a larger
-// maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 51 and
+// maximum arrives; the backward reads them once more and writes the gradient (16384 x 8192 bf16, one after the other: 52 and
 // 83 us, 805 MB at 6.0 TB/s, a part of the logits from the last-level cache).  Sums are f32; exponents are of x - m <= 0.
 // Masked logits (-inf) have p = 0, so by the formula no gradient, except a masked token in a row that allows others: logp -inf,
 // and dlogp at its place.  A row of nothing but -inf has no distribution: logp -inf, H 0, gradient 0.  A

@@ -8,8 +8,8 @@
 // variance is that of the centred values (no cancellation of sum(x^2) - mu^2) at no second read.  All sums are f32; the mean of
 // the centred values, which is what the first mean's rounding left in them, is taken off them again: constant rows are exactly
 // centred and y = b, where a mean one step off would be raised by r, up to 316 at eps = 1e-5.
-// 16384 x 512 bf16: forward 10.3 us (3.3 TB/s; 9.4 without the second mean), backward 13.2 us (3.8 TB/s) and 3.8 us for the column
-// sums; 65536 x 128 f32 forward 14.8 us (4.5 TB/s; 13.6), where the launch's own few us weigh less.
+// 16384 x 512 bf16: forward 10.3 us alone (3.3 TB/s; 9.4 without the second mean), 11.6 in a training pass, backward 13.5 us (3.7
+// TB/s) and 3.9 us for the column sums; 65536 x 128 f32 forward 14.8 us (4.5 TB/s; 13.6), where the launch's own few us weigh less.
 #include "common.h"
 #include "rows.h"
 
