@@ -332,3 +332,24 @@ def test_layer_norm_without_a_gradient_of_x(c, dt):
     (dw, db), less = grads(x, (w, b))
     assert more - less >= x.numel() * x.element_size()
     assert torch.equal(dw, full[1]) and torch.equal(db, full[2])
+
+
+def test_adamw_8bit_stochastic_rounding_beyond_the_cache():
+    """Buffers over 256 MiB take the streaming kernel: the same bits at the same places as in a small buffer."""
+    from test_gpu_token_ops import make_opt
+    n = 999_936                                                     # whole blocks
+    big, g = make_opt(8, shapes=[(17_000_001,)], rounding="stochastic")
+    small, _ = make_opt(8, shapes=[(n,)], rounding="stochastic")
+    small.flat_p.copy_(big.flat_p[:n])
+    for _ in range(3):
+        big.zero_grad()
+        big.params[0].grad.add_(torch.randn(17_000_001, device="cuda", generator=g) * 1e-3)
+        small.flat_g.copy_(big.flat_g[:n])
+        big.step(), small.step()
+    # one parameter of one dimension in both: neither is decayed
+    assert torch.equal(big.flat_p[:n], small.flat_p)
+    for name in ("exp_avg", "root_sq"):
+        assert torch.equal(getattr(big, name)[:n].view(torch.uint8), getattr(small, name).view(torch.uint8)), name
+    for name in ("exp_avg_scale", "root_sq_scale"):
+        assert torch.equal(getattr(big, name)[:n // 256], getattr(small, name)), name
+    assert torch.isfinite(big.flat_p).all() and not big.flat_p[17_000_001:].any()
